@@ -285,7 +285,9 @@ DEVI void unpack_f16x8(const u32x4 q, float (&x)[8]) {
 // ---- hand-picked instructions for the row passes.  The student-row loop is VALU-bound (timing-only build without
 // the gradient stores: 162 of 193 us), so its instruction count IS its speed: hipcc spends ~13.7 VALU
 // instructions per logit (separate f16 -> f32 conversions, canonicalising v_max before every fmaxf, scalar
-// fma / add where the packed-f32 forms do two lanes' worth per issue); these forms need ~8.
+// fma / add); these forms need ~8.  The pairs below are two single instructions each: the packed fp32 forms
+// have given wrong values on this chip now and then, so nothing here is built with them.  Sums, differences and
+// products stay single instructions (asm) so that no fma contraction changes their rounding.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 DEVI float max3_raw(float a, float b, float c) {           // no canonicalisation, NaNs not expected
     float r;
@@ -293,19 +295,19 @@ DEVI float max3_raw(float a, float b, float c) {           // no canonicalisatio
     return r;
 }
 DEVI f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) {
-    f32x2 r;
-    asm("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
+    return f32x2{__builtin_fmaf(a.x, b.x, c.x), __builtin_fmaf(a.y, b.y, c.y)};
 }
 DEVI f32x2 pk_add(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+    float x, y;
+    asm("v_add_f32 %0, %1, %2" : "=v"(x) : "v"(a.x), "v"(b.x));
+    asm("v_add_f32 %0, %1, %2" : "=v"(y) : "v"(a.y), "v"(b.y));
+    return f32x2{x, y};
 }
 DEVI f32x2 pk_sub(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+    float x, y;
+    asm("v_sub_f32 %0, %1, %2" : "=v"(x) : "v"(a.x), "v"(b.x));
+    asm("v_sub_f32 %0, %1, %2" : "=v"(y) : "v"(a.y), "v"(b.y));
+    return f32x2{x, y};
 }
 // f16 half of e times f32 b PLUS the same f16 half of q
 template <bool HI> DEVI float mix_h_f_h(unsigned e, float b, unsigned q) {
@@ -320,9 +322,10 @@ DEVI float dot2_h(unsigned a, unsigned b, float c) {      // a.lo * b.lo + a.hi 
     return r;
 }
 DEVI f32x2 pk_mul(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("v_pk_mul_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+    float x, y;
+    asm("v_mul_f32 %0, %1, %2" : "=v"(x) : "v"(a.x), "v"(b.x));
+    asm("v_mul_f32 %0, %1, %2" : "=v"(y) : "v"(a.y), "v"(b.y));
+    return f32x2{x, y};
 }
 // f16 half (HI: upper) of word h, times f32 b, plus f32 c -- no separate conversion
 template <bool HI> DEVI float mix_h_f_f(unsigned h, float b, float c) {
