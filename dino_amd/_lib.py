@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libdino_hip.so")
 
 DINO_F32, DINO_BF16 = 0, 1
 DINO_CHUNK = 8192
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 
 class GemmArgs(ctypes.Structure):
@@ -66,6 +66,9 @@ SIGNATURES = {
     "dino_loss_fwd_bwd": [I, P, P, P, P, P, P, P, I, I, I, F, F, P],
     "dino_center_update": [P, P, I, F, F, P, I, P, P],
     "dino_proto_loss_chunk": [I, I, P, L, P, L, P, P, P, I, I, I, I, I, F, F, P, P, P],
+    "dino_logprob_workspace": [L, I, I, ctypes.POINTER(c_int64)],
+    "dino_logprob_fwd": [I, P, L, L, I, P, F, P, I, I, P, P, P, P, P, P, L, P],
+    "dino_logprob_bwd": [I, P, L, L, I, P, F, P, P, P, I, P, P, P, I, P, P, L, P],
     "dino_grad_sqnorm": [P, P, I, P, P],
     "dino_clip_coef": [P, P, I, P, F, P, P, P, P],
     "dino_grad_scale": [P, P, I, P, P],

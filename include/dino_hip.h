@@ -257,6 +257,31 @@ int dino_proto_loss_chunk(int dtype, int phase, void* s_chunk, int64_t lds, cons
                           float* loss_parts, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Log probabilities of given prototypes, entropy and best prototypes of rows of logits, and their gradient (no
+ * counterpart in the reference, which only forms the loss; what one looks at, or distils from, beside it).
+ * With d = logits - center (center nullable, fp32 [K]) and z = d * inv_temp, per row:
+ *   log_prob [rows, T]  log softmax(z) at targets [rows, T] (int64; -1: no target, 0; anything else outside [0, K): NaN)
+ *   entropy  [rows]     -sum p log p (natural logarithm)
+ *   stats    [rows, 2]  (max d, log sum exp(z - max z)): what the gradient needs
+ *   top_index / top_log_prob [rows, topk]  the largest d, equal ones by their index (topk <= 64, 0: none)
+ * logits: dtype [rows, K], row stride ld (any; rows need no alignment beyond the element's).  -inf logits have
+ * probability 0; a row of nothing else gives log_prob -inf, entropy 0 and gradient 0.  NaN or +inf: NaN for the row.
+ * K <= 1048576 (else DINO_ERR_TOO_LARGE).  workspace: dino_logprob_workspace bytes (0 for K <= 4096), of this call alone.
+ * Backward: dlogits [rows, K] (row stride ldd, may be logits itself) = gradient of
+ *   sum dlog_prob * log_prob + sum dentropy * entropy + sum dtop_log_prob * top_log_prob   (each nullable),
+ * rounded to dtype once.  center is a constant.  T <= 4096.
+ * ------------------------------------------------------------------------------------------ */
+int dino_logprob_workspace(int64_t rows, int K, int topk, int64_t* bytes /* host */);
+int dino_logprob_fwd(int dtype, const void* logits, int64_t ld, int64_t rows, int K, const float* center,
+                     float inv_temp, const int64_t* targets, int T, int topk, float* log_prob, float* entropy,
+                     float* stats, float* top_log_prob, int64_t* top_index, void* workspace, int64_t workspace_bytes,
+                     void* stream);
+int dino_logprob_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int K, const float* center,
+                     float inv_temp, const float* stats, const float* entropy, const int64_t* targets, int T,
+                     const float* dlog_prob, const float* dentropy, const int64_t* top_index, int topk,
+                     const float* dtop_log_prob, void* dlogits, int64_t ldd, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Flat-buffer optimiser kernels.  All student parameters live in one fp32 buffer (each
  * nn.Parameter is a view), likewise grads, AdamW moments and the teacher copy.
  * chunk table: int64 [nchunks, 3] = (tensor index, start element, length<=DINO_CHUNK).
