@@ -48,6 +48,19 @@ template <> DEVI void store8u<bf16>(bf16* p, const float (&v)[8]) {
     *(bf16x8u*)p = a;
 }
 
+// eight elements as loaded: kept packed while they are in flight
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+    bf16x8u v;
+    DEVI void load(const bf16* p) { v = *(const bf16x8u*)p; }
+    DEVI float at(int i) const { return (float)v[i]; }
+};
+template <> struct Raw8<float> {
+    f32x4u lo, hi;
+    DEVI void load(const float* p) { lo = *(const f32x4u*)p; hi = *(const f32x4u*)(p + 4); }
+    DEVI float at(int i) const { return i < 4 ? lo[i & 3] : hi[i & 3]; }
+};
+
 // order-preserving bits: a < b  <=>  ord(a) < ord(b); -0 counts as +0, every NaN above +inf
 DEVI unsigned ord_bits(float d) {
     const unsigned b = __builtin_bit_cast(unsigned, d + 0.f);
@@ -122,7 +135,7 @@ DEVI void put_top(const FwdArgs& a, int64_t row, int j, u64 key, float md, float
 
 // One workgroup of NT threads takes one chunk (at most NT * 8 * NV columns) of one row, held in registers: read
 // once, then the maximum, the sums and the best k come from registers.
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool CEN>
 __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
     constexpr int NW = NT / 64;
     __shared__ float red[3 * NW];
@@ -137,37 +150,51 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
     const T* x = (const T*)a.x + row * a.ld;
 
     float d[NV][8];
-    float tm = NEG_INF;
+    if (c0 + NT * 8 * NV <= c1) {        // a whole chunk: no column behind the end
+        Raw8<T> raw[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int at = c0 + (j * NT + tid) * 8;
-        if (at + 8 <= c1) {
-            load8u<T>(x + at, d[j]);
+        for (int j = 0; j < NV; ++j) raw[j].load(x + c0 + (j * NT + tid) * 8);
+        if (CEN) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                float c[8];
+                load8u<float>(a.center + c0 + (j * NT + tid) * 8, c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[j][i] = raw[j].at(i) - c[i];
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[j][i] = at + i < c1 ? to_f32<T>(x[at + i]) : NEG_INF;
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[j][i] = raw[j].at(i);
         }
-    }
-    if (a.center) {
+    } else {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int at = c0 + (j * NT + tid) * 8;
             if (at + 8 <= c1) {
-                float c[8];
-                load8u<float>(a.center + at, c);
+                load8u<T>(x + at, d[j]);
+                if (CEN) {
+                    float c[8];
+                    load8u<float>(a.center + at, c);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[j][i] -= c[i];
+                    for (int i = 0; i < 8; ++i) d[j][i] -= c[i];
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (at + i < c1) d[j][i] -= a.center[at + i];
+                    d[j][i] = at + i < c1 ? to_f32<T>(x[at + i]) - (CEN ? a.center[at + i] : 0.f) : NEG_INF;
             }
         }
     }
+    float vm[NV], tm = NEG_INF;                                    // NaNs pass by: they show in the sums
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        vm[j] = d[j][0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tm = fmaxf(tm, d[j][i]);       // NaNs pass by: they show in the sums
+        for (int i = 1; i < 8; ++i) vm[j] = fmaxf(vm[j], d[j][i]);
+        tm = fmaxf(tm, vm[j]);
+    }
 
     float md = wave_max(tm);
     if (NW > 1) {
@@ -176,17 +203,35 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
 #pragma unroll
         for (int w = 0; w < NW; ++w) md = fmaxf(md, red[w]);
     }
-    const float ref = md == NEG_INF ? 0.f : md, sc = a.inv_temp * LOG2E;
+    // (d - ref) / tau in units of log 2.  One fma an element: z = d sc - fl(ref sc), whose offset against the exact
+    // (d - ref) sc is the same dz for every element of the chunk and is taken out of the sums below.  Where ref sc
+    // itself is out of range (rows of the type's lowest value) the difference is formed first.
+    const float ref = md == NEG_INF ? 0.f : md, sc = a.inv_temp * LOG2E, off = ref * sc;
     float s = 0.f, t2 = 0.f;
+    if (fabsf(off) < 1e30f) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float z = (d[j][i] - ref) * sc;
-            const float e = __builtin_amdgcn_exp2f(z);
-            s += e;
-            t2 = fmaf(e, fmaxf(z, Z_MIN), t2);                     // e = 0 meets z = -inf
-        }
+            for (int i = 0; i < 8; ++i) {
+                const float z = fmaf(d[j][i], sc, -off);
+                const float e = __builtin_amdgcn_exp2f(z);
+                s += e;
+                t2 = fmaf(e, fmaxf(z, Z_MIN), t2);                 // e = 0 meets z = -inf
+            }
+        const float dz = fmaf(ref, sc, -off), f = __builtin_amdgcn_exp2f(-dz);
+        t2 = f * fmaf(-dz, s, t2);
+        s *= f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float z = (d[j][i] - ref) * sc;
+                const float e = __builtin_amdgcn_exp2f(z);
+                s += e;
+                t2 = fmaf(e, fmaxf(z, Z_MIN), t2);
+            }
+    }
     s = wave_sum(s);
     t2 = wave_sum(t2);
     if (NW > 1) {
@@ -217,20 +262,23 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
             for (int w = 0; w < NW; ++w) th = max(th, __builtin_bit_cast(unsigned, red[w]));
         }
         const float T_ = th <= 0x007Fu ? NEG_INF : ord_float(th << 16);
+        const bool nan = s != s;             // a NaN is no maximum of its vector: such a chunk takes the rounds below
         // (columns behind the chunk's end hold -inf and are told by their index)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int at = c0 + (j * NT + tid) * 8;
+            if (vm[j] >= T_ && !nan) {
+                const int at = c0 + (j * NT + tid) * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!(d[j][i] < T_) && at + i < c1) {
-                    const int p = atomicAdd(&ncand, 1);
-                    if (p < CAP) cand[p] = make_key(d[j][i], at + i);
-                }
+                for (int i = 0; i < 8; ++i)
+                    if (d[j][i] >= T_ && at + i < c1) {
+                        const int p = atomicAdd(&ncand, 1);
+                        if (p < CAP) cand[p] = make_key(d[j][i], at + i);
+                    }
+            }
         }
         __syncthreads();
         const int n = ncand;
-        if (n <= CAP) {
+        if (n <= CAP && !nan) {
             for (int q = tid; q < MAX_K; q += NT) best[q] = 0;
             __syncthreads();
             for (int q = tid; q < n; q += NT) {
@@ -240,18 +288,13 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
                 if (rank < k) best[rank] = key;
             }
             __syncthreads();
-        } else {                     // many equal or masked values: k rounds of the next best key
+        } else {      // many equal or masked values, or a NaN: k rounds of the next best key, columns read again
             u64 last = ~0ull;
             for (int q = 0; q < k; ++q) {
                 u64 mine = 0;
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int at = c0 + (j * NT + tid) * 8;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const u64 key = at + i < c1 ? make_key(d[j][i], at + i) : 0;
-                        if (key < last && key > mine) mine = key;
-                    }
+                for (int at = c0 + tid; at < c1; at += NT) {
+                    const u64 key = make_key(to_f32<T>(x[at]) - (a.center ? a.center[at] : 0.f), at);
+                    if (key < last && key > mine) mine = key;
                 }
                 mine = wave_max_u64(mine);
                 if (NW > 1) {
@@ -424,18 +467,18 @@ __global__ __launch_bounds__(BNT) void logprob_bwd_kernel(const BwdArgs a) {
     }
 }
 
-// Columns per workgroup.  A row of up to 4096 columns is one wave's; longer ones are cut into chunks of at most
-// 16384 that a second kernel joins.
+// Columns per workgroup: 32 a thread (64 where 64 chunks of 8192 would not reach the end).  Rows of up to
+// 8192 columns are one workgroup's (one wave's up to 2048); longer ones are cut into chunks that a second kernel joins.
 struct Plan {
     int nt, nv, chunk, S;
 };
 Plan plan_of(int64_t rows, int K) {
     Plan p;
-    p.nt = K <= 4096 ? 64 : 256;
+    p.nt = K <= 2048 ? 64 : K <= 4096 ? 128 : 256;
     p.nv = 1;
-    const int most = 8;
+    const int most = K <= 8192 * MAX_CHUNKS ? 4 : 8;
     while (p.nv < most && p.nt * 8 * p.nv < K) p.nv *= 2;
-    // few rows: shorter chunks, so that the row is read by many CUs
+    // few rows: shorter chunks, so that a row is read by many CUs
     if (K > 4096)
         while (p.nv > 1) {
             const int64_t next = (K + p.nt * 4 * p.nv - 1) / (p.nt * 4 * p.nv);
@@ -447,14 +490,14 @@ Plan plan_of(int64_t rows, int K) {
     return p;
 }
 
-template <typename T> int run_fwd(FwdArgs a, const Plan& p, hipStream_t st) {
+template <typename T, bool CEN> int run_fwd(const FwdArgs& a, const Plan& p, hipStream_t st) {
     const dim3 grid((unsigned)(a.rows * p.S));
 #define LAUNCH(NT_, NV_) \
-    if (p.nt == NT_ && p.nv == NV_) hipLaunchKernelGGL((logprob_fwd_kernel<T, NT_, NV_>), grid, dim3(NT_), 0, st, a)
+    if (p.nt == NT_ && p.nv == NV_) hipLaunchKernelGGL((logprob_fwd_kernel<T, NT_, NV_, CEN>), grid, dim3(NT_), 0, st, a)
     LAUNCH(64, 1);
     LAUNCH(64, 2);
     LAUNCH(64, 4);
-    LAUNCH(64, 8);
+    LAUNCH(128, 4);
     LAUNCH(256, 1);
     LAUNCH(256, 2);
     LAUNCH(256, 4);
@@ -494,12 +537,15 @@ extern "C" int dino_logprob_fwd(int dtype, const void* logits, int64_t ld, int64
                    (topk == 0 || (top_log_prob && top_index)));
     if (K > CHUNK_MAX * MAX_CHUNKS) return DINO_ERR_TOO_LARGE;
     const Plan p = plan_of(rows, K);
-    if (rows >= (1ll << 31) || rows * p.S * p.nt >= (1ll << 32)) return DINO_ERR_TOO_LARGE;   // threads of one launch
+    // fewer than 2^32 threads a launch (the joining kernel: 64 a row)
+    if (rows >= (1ll << 26) || rows * p.S * p.nt >= (1ll << 32)) return DINO_ERR_TOO_LARGE;
     DINO_CHECK_ARG(p.S == 1 || (workspace && workspace_bytes >= ws_bytes(rows, K, topk)));
     FwdArgs a{logits, ld, rows, K, p.S, p.chunk, T, topk, center, inv_temp, targets, log_prob, entropy, stats,
               top_log_prob, top_index, (Part*)workspace,
               p.S > 1 ? (u64*)((char*)workspace + rows * p.S * (int64_t)sizeof(Part)) : nullptr};
-    return dtype == DINO_BF16 ? run_fwd<bf16>(a, p, (hipStream_t)stream) : run_fwd<float>(a, p, (hipStream_t)stream);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == DINO_BF16) return center ? run_fwd<bf16, true>(a, p, st) : run_fwd<bf16, false>(a, p, st);
+    return center ? run_fwd<float, true>(a, p, st) : run_fwd<float, false>(a, p, st);
 }
 
 extern "C" int dino_logprob_bwd(int dtype, const void* logits, int64_t ld, int64_t rows, int K, const float* center,

@@ -4,6 +4,7 @@ can take the whole GPU down), raw device pointers + the current HIP stream into 
 PyTorch is only the allocator / stream provider here; every computation is a HIP kernel.
 """
 import ctypes
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -22,7 +23,29 @@ def dt_code(dtype) -> int:
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (torch.cuda.current_stream() builds a Stream object: 2.8 us a call against 0.1)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return None
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on(device):
+    """Context in which `device` is the current one: tensors of another GPU than the current one run on THEIR device's
+    current stream."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _p(t):
@@ -442,49 +465,54 @@ LOGPROB_MAX_TOPK, LOGPROB_MAX_TARGETS = 64, 4096
 
 
 def _logprob_operands(logits, targets, center, temp):
-    """(rows, K, T, inverse temperature) of checked operands."""
+    """(rows, K, T, row stride, inverse temperature) of checked operands."""
     _dev(logits, targets, center)
-    _req(logits.dim() == 2 and logits.shape[1] > 0 and logits.stride(1) == 1, "logits [R, K], columns side by side",
-         tuple(logits.shape), logits.stride())
+    _req(logits.dim() == 2, "logits: [R, K]", logits.shape)
     R, K = logits.shape
-    _req(R <= 1 or logits.stride(0) >= K, "rows overlap", logits.stride())
+    ld, one = logits.stride()
+    _req(K > 0 and (one == 1 or K == 1), "logits: columns side by side", logits.shape, logits.stride())
+    _req(R <= 1 or ld >= K, "logits: rows overlap", logits.stride())
     T = 0
     if targets is not None:
-        _req(targets.dtype == torch.int64 and targets.dim() == 2 and targets.shape[0] == R and targets.is_contiguous(),
-             "targets: contiguous int64 [R, T]", targets.dtype, tuple(targets.shape))
+        _req(targets.dtype is torch.int64 and targets.dim() == 2 and targets.shape[0] == R and targets.is_contiguous(),
+             "targets: contiguous int64 [R, T]", targets.dtype, targets.shape)
         T = targets.shape[1]
         _req(T <= LOGPROB_MAX_TARGETS, f"at most {LOGPROB_MAX_TARGETS} targets a row", T)
+        _req(targets.device == logits.device, "operands on different devices")
     if center is not None:
-        _f32(center)
-        _req(center.numel() == K, "center: one value a column", tuple(center.shape), K)
-    for t in (targets, center):
-        _req(t is None or t.device == logits.device, "operands on different devices")
-    _req(isinstance(temp, (int, float)) and 0.0 < temp < float("inf"), "temperature must be positive", temp)
-    inv = 1.0 / float(temp)
-    _req(1e-37 < inv < 1e37, "temperature out of range", temp)
-    return R, K, T, inv
+        _req(center.dtype is torch.float32 and center.is_contiguous() and center.numel() == K,
+             "center: contiguous float32, one value a column", center.dtype, center.shape)
+        _req(center.device == logits.device, "operands on different devices")
+    _req(isinstance(temp, (int, float)) and 1e-37 < temp < 1e37, "temperature: positive and finite", temp)
+    return R, K, T, max(ld, K), 1.0 / temp
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprob_workspace(R, K, topk):
+    need = ctypes.c_int64(0)
+    check(_lib.load().dino_logprob_workspace(R, K, topk, ctypes.byref(need)), "dino_logprob_workspace")
+    return need.value
 
 
 def logprob_fwd(logits, targets=None, *, center=None, temp=1.0, topk=0) -> LogProbs:
     """Log probabilities, entropy and best columns of softmax((logits - center) / temp), one pass over the logits
     (include/dino_hip.h: dino_logprob_fwd).  logits [R, K] bf16 / fp32 with any row stride; targets int64 [R, T]
     (-1: none) or None; center fp32 [K] or None."""
-    R, K, T, inv = _logprob_operands(logits, targets, center, temp)
+    R, K, T, ld, inv = _logprob_operands(logits, targets, center, temp)
     _req(isinstance(topk, int) and 0 <= topk <= min(K, LOGPROB_MAX_TOPK),
          f"topk between 0 and min(K, {LOGPROB_MAX_TOPK})", topk)
-    dev = logits.device
-    with torch.cuda.device(dev):
-        lp = torch.empty((R, T), dtype=torch.float32, device=dev)
-        ent = torch.empty(R, dtype=torch.float32, device=dev)
-        stats = torch.empty((R, 2), dtype=torch.float32, device=dev)
-        tlp = torch.empty((R, topk), dtype=torch.float32, device=dev) if topk else None
+    dt, dev, f32 = dt_code(logits.dtype), logits.device, torch.float32
+    need = _logprob_workspace(R, K, topk)
+    with _on(dev):
+        lp = torch.empty((R, T), dtype=f32, device=dev)
+        ent = torch.empty((R,), dtype=f32, device=dev)
+        stats = torch.empty((R, 2), dtype=f32, device=dev)
+        tlp = torch.empty((R, topk), dtype=f32, device=dev) if topk else None
         tix = torch.empty((R, topk), dtype=torch.int64, device=dev) if topk else None
-        need = ctypes.c_int64(0)
-        check(_lib.load().dino_logprob_workspace(R, K, topk, ctypes.byref(need)), "dino_logprob_workspace")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        check(_lib.load().dino_logprob_fwd(dt_code(logits.dtype), _p(logits), max(logits.stride(0), K), R, K, _p(center),
-                                           inv, _p(targets), T, topk, _p(lp), _p(ent), _p(stats), _p(tlp), _p(tix),
-                                           _p(ws), need.value, _stream()), "dino_logprob_fwd")
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        check(_lib.load().dino_logprob_fwd(dt, logits.data_ptr(), ld, R, K, _ptr(center), inv, _ptr(targets), T, topk,
+                                           lp.data_ptr(), ent.data_ptr(), stats.data_ptr(), _ptr(tlp), _ptr(tix),
+                                           _ptr(ws), need, _stream()), "dino_logprob_fwd")
     return LogProbs(lp, ent, stats, tlp, tix)
 
 
@@ -493,28 +521,28 @@ def logprob_bwd(logits, fwd: LogProbs, *, targets=None, center=None, temp=1.0, d
     """Gradient of logprob_fwd's log_prob / entropy / top_log_prob with respect to the logits, given theirs (each may be
     None).  logits, targets, center and temp as in the forward call; dlogits may be a buffer of the caller's (the
     logits themselves too)."""
-    R, K, T, inv = _logprob_operands(logits, targets, center, temp)
-    k = 0 if fwd.top_index is None else fwd.top_index.shape[1]
-    _dev(fwd.entropy, fwd.stats, fwd.top_index, dlog_prob, dentropy, dtop_log_prob, dlogits)
-    _f32(fwd.entropy, fwd.stats, dlog_prob, dentropy, dtop_log_prob)
-    _req(fwd.stats.shape == (R, 2) and fwd.entropy.shape == (R,), "forward results of other logits")
+    R, K, T, ld, inv = _logprob_operands(logits, targets, center, temp)
+    ent, stats, tix = fwd.entropy, fwd.stats, fwd.top_index
+    k = 0 if tix is None else tix.shape[1]
+    dev = logits.device
+    _dev(ent, stats, tix, dlog_prob, dentropy, dtop_log_prob, dlogits)
+    _f32(ent, stats, dlog_prob, dentropy, dtop_log_prob)
+    _req(stats.shape == (R, 2) and ent.shape == (R,), "forward results of other logits")
     _req(dlog_prob is None or (targets is not None and dlog_prob.shape == (R, T)), "dlog_prob: [R, T], with its targets")
     _req(dentropy is None or dentropy.shape == (R,), "dentropy: [R]")
     _req(dtop_log_prob is None or (k > 0 and dtop_log_prob.shape == (R, k)), "dtop_log_prob: [R, topk]")
-    _req(fwd.top_index is None or (fwd.top_index.dtype == torch.int64 and fwd.top_index.is_contiguous()
-                                   and fwd.top_index.shape[0] == R))
-    dev = logits.device
-    for t in (fwd.entropy, fwd.stats, fwd.top_index, dlog_prob, dentropy, dtop_log_prob, dlogits):
+    _req(tix is None or (tix.dtype is torch.int64 and tix.is_contiguous() and tix.shape[0] == R), "top_index")
+    for t in (ent, stats, tix, dlog_prob, dentropy, dtop_log_prob, dlogits):
         _req(t is None or t.device == dev, "operands on different devices")
-    with torch.cuda.device(dev):
+    with _on(dev):
         if dlogits is None:
             dlogits = torch.empty((R, K), dtype=logits.dtype, device=dev)
-        _req(dlogits.shape == (R, K) and dlogits.dtype == logits.dtype and dlogits.stride(1) == 1
+        _req(dlogits.shape == (R, K) and dlogits.dtype == logits.dtype and (dlogits.stride(1) == 1 or K == 1)
              and (R <= 1 or dlogits.stride(0) >= K), "dlogits: [R, K] of the logits' type")
         check(_lib.load().dino_logprob_bwd(
-            dt_code(logits.dtype), _p(logits), max(logits.stride(0), K), R, K, _p(center), inv, _p(fwd.stats),
-            _p(fwd.entropy), _p(targets), T, _p(dlog_prob), _p(dentropy), _p(fwd.top_index), k, _p(dtop_log_prob),
-            _p(dlogits), max(dlogits.stride(0), K), _stream()), "dino_logprob_bwd")
+            dt_code(logits.dtype), logits.data_ptr(), ld, R, K, _ptr(center), inv, stats.data_ptr(), ent.data_ptr(),
+            _ptr(targets), T, _ptr(dlog_prob), _ptr(dentropy), _ptr(tix), k, _ptr(dtop_log_prob), dlogits.data_ptr(),
+            max(dlogits.stride(0), K), _stream()), "dino_logprob_bwd")
     return dlogits
 
 
