@@ -40,6 +40,14 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class OrthoItem(ctypes.Structure):
+    _fields_ = [
+        ("inp", c_void_p), ("out", c_void_p),
+        ("in_batch", c_int64), ("in_ld", c_int64), ("out_batch", c_int64), ("out_ld", c_int64),
+        ("rows", c_int32), ("cols", c_int32), ("batch", c_int32), ("dtype", c_int32),
+    ]
+
+
 P, I, L, F = c_void_p, c_int, c_int64, c_float
 
 # name -> argtypes; every function returns int (0 = OK)
@@ -73,6 +81,8 @@ SIGNATURES = {
     "dino_clip_coef": [P, P, I, P, F, P, P, P, P],
     "dino_grad_scale": [P, P, I, P, P],
     "dino_adamw_ema": [P, P, P, P, P, P, P, P, I, P, P, F, F, F, F, F, P],
+    "dino_ortho_workspace": [ctypes.POINTER(OrthoItem), I, ctypes.POINTER(c_int64)],
+    "dino_ortho": [ctypes.POINTER(OrthoItem), I, I, ctypes.POINTER(c_float), ctypes.c_double, P, L, P],
     "dino_ema": [P, P, P, L, F, F, P],
     "dino_cast_bf16": [P, P, L, P],
     "dino_transpose_batched": [I, P, P, P, I, P],

@@ -575,6 +575,57 @@ def adamw_ema(param, grad, exp_avg, exp_avg_sq, teacher, param_shadow, teacher_s
           "dino_adamw_ema")
 
 
+NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic that takes singular values of (0, 1] near 1 in five steps
+ORTHO_MAX_STEPS = 16
+
+
+def orthogonalize(updates, *, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
+    """Orthogonalised updates by Newton-Schulz products (include/dino_hip.h: dino_ortho), all matrices in one sequence of
+    launches.  updates: a tensor or a list of tensors, each [rows, cols] or [batch, rows, cols] in fp32 / bf16, columns
+    side by side, rows with any stride.  coeffs: (a, b, c), or one such triple per step.  Returns bf16 tensors of the same
+    shapes (a tensor for a tensor, a list for a list); out: the caller's own, in the same form."""
+    single = isinstance(updates, torch.Tensor)
+    ups = [updates] if single else list(updates)
+    _req(isinstance(steps, int) and 1 <= steps <= ORTHO_MAX_STEPS, f"steps: 1 to {ORTHO_MAX_STEPS}", steps)
+    rows = [tuple(c) for c in coeffs] if len(coeffs) and not isinstance(coeffs[0], (int, float)) else [tuple(coeffs)] * steps
+    _req(len(rows) == steps and all(len(c) == 3 for c in rows), "coeffs: (a, b, c), or one triple per step", coeffs)
+    _req(isinstance(eps, (int, float)) and 0.0 <= eps < 1e30, "eps", eps)
+    if not ups:
+        return []
+    outs = [None] * len(ups) if out is None else ([out] if single else list(out))
+    _req(len(outs) == len(ups), "out: one for each update")
+    _dev(*ups, *outs)
+    dev = ups[0].device
+    items = (_lib.OrthoItem * len(ups))()
+    res = []
+    with _on(dev):
+        for q, u, o in zip(items, ups, outs):
+            _req(u.dim() in (2, 3) and u.device == dev, "updates: [rows, cols] or [batch, rows, cols] on one device", u.shape)
+            if o is None:
+                o = torch.empty(u.shape, dtype=torch.bfloat16, device=dev)
+            _req(o.shape == u.shape and o.dtype is torch.bfloat16 and o.device == dev, "out: bf16 of the update's shape")
+            r, c = u.shape[-2:]
+            for t in (u, o):
+                _req(r > 0 and c > 0 and (t.stride(-1) == 1 or c == 1) and (t.stride(-2) >= c or r == 1),
+                     "columns side by side, rows apart", t.shape, t.stride())
+                _req(t.dim() == 2 or t.shape[0] <= 1 or t.stride(0) >= (r - 1) * t.stride(1) + c, "matrices overlap", t.stride())
+            q.inp, q.out = u.data_ptr(), o.data_ptr()
+            q.rows, q.cols, q.dtype = r, c, dt_code(u.dtype)
+            q.in_ld, q.out_ld = max(u.stride(-2), c), max(o.stride(-2), c)
+            if u.dim() == 3:
+                q.batch, q.in_batch, q.out_batch = u.shape[0], u.stride(0), o.stride(0)
+            else:
+                q.batch = 1
+            res.append(o)
+        cf = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
+        need = ctypes.c_int64(0)
+        lib = _lib.load()
+        check(lib.dino_ortho_workspace(items, len(ups), ctypes.byref(need)), "dino_ortho_workspace")
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
+        check(lib.dino_ortho(items, len(ups), steps, cf, float(eps), ws.data_ptr(), need.value, _stream()), "dino_ortho")
+    return res[0] if single else res
+
+
 def ema(teacher, student, teacher_shadow, m, one_minus_m):
     _dev(teacher, student, teacher_shadow)
     _f32(teacher, student)
