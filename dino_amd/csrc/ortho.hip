@@ -13,6 +13,9 @@
 // products hi hi + hi lo + lo hi, three passes of the same loop); after that plain fp16.  On an update of four strong
 // directions over noise the result is then 0.003 off 64 bits, with plain fp16 throughout 0.04, with bf16 0.33.
 #include <math.h>
+#include <stdlib.h>
+
+#include <type_traits>
 
 #include "common.h"
 
@@ -24,9 +27,7 @@ typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
-constexpr int TILE = 128, BK = 32, S = 4, NTHR = 256;
-constexpr int OPB = TILE * BK * 2;              // bytes of one operand's stage
-constexpr int STAGE = 2 * OPB;                  // 16 KB
+constexpr int BK = 32, NTHR = 256;
 constexpr int ITEMS = 16;                       // items described by one launch of the norm kernel
 constexpr float SX = 4096.f;                    // X is stored times this
 constexpr double SPLIT_ABOVE = 16.0;
@@ -39,7 +40,7 @@ struct Mat {
     int rows, cols, batch, dtype;
     int tall, m, n, mp, np;                     // m <= n; mp, np: padded to 32 (zeros)
     int parts, part0, mat0;                     // partial sums of the norm: per matrix, first index; first matrix
-    int tm, tn, sym0, rect0, prep0, ntiles_sym; // tiles of 128; first global tile of each kind
+    int sym0, rect0, prep0, nsym, nrect;        // first global tile of each kind; tiles of the whole item
 };
 struct Setup {
     Mat it[ITEMS];
@@ -54,17 +55,6 @@ struct Ws {                                     // regions of the workspace
     f16 *x[2][2], *a[2], *b[2];                 // [buffer][hi / lo]
 };
 
-DEVI void split_store(f16* hi, f16* lo, const float (&v)[4]) {
-    f16x4 h, l;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        h[r] = (f16)v[r];
-        l[r] = (f16)(v[r] - (float)h[r]);
-    }
-    *(f16x4*)hi = h;
-    if (lo) *(f16x4*)lo = l;
-}
-
 DEVI double block_sum_f64(double v, double* red) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
@@ -76,14 +66,29 @@ DEVI double block_sum_f64(double v, double* red) {
     return r;
 }
 
-template <typename T> DEVI double row_range_sq(const T* p, int64_t ld, int cols, int64_t e0, int64_t e1) {
+// squares of rows [r0, r1): a wave a row; V elements a lane and load
+template <typename T, int V> DEVI double rows_sq(const T* p, int64_t ld, int cols, int r0, int r1) {
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T) * V)));
+    const int lane = threadIdx.x & 63;
     double s = 0;
-    for (int64_t e = e0 + threadIdx.x; e < e1; e += NTHR) {
-        const int64_t r = e / cols;
-        const double x = (double)to_f32<T>(p[r * ld + (e - r * cols)]);
-        s += x * x;
+    for (int r = r0 + (threadIdx.x >> 6); r < r1; r += NTHR / 64) {
+        const T* x = p + r * ld;
+        for (int c = lane * V; c < cols; c += 64 * V) {
+            if (V == 1 || c + V <= cols) {
+                const vec v = *(const vec*)(x + c);
+#pragma unroll
+                for (int i = 0; i < V; ++i) { const double d = (double)(float)v[i]; s = fma(d, d, s); }
+            } else {
+                for (int i = c; i < cols; ++i) { const double d = (double)(float)x[i]; s = fma(d, d, s); }
+            }
+        }
     }
     return s;
+}
+template <typename T> DEVI double rows_sq(const void* in, int64_t at, int64_t ld, int cols, int r0, int r1) {
+    const T* p = (const T*)in + at;
+    if (((uintptr_t)p | (uint64_t)(ld * sizeof(T))) % (4 * sizeof(T)) == 0) return rows_sq<T, 4>(p, ld, cols, r0, r1);
+    return rows_sq<T, 1>(p, ld, cols, r0, r1);
 }
 
 // Partial sums of squares (fp64: neither 1e-30 nor 1e30 leaves the range), and the item table with the tile -> item maps
@@ -96,16 +101,14 @@ __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const 
     const int w = blockIdx.x - su.wg0[i], nw = su.wg0[i + 1] - su.wg0[i], id = su.first + i;
     if (w == 0 && threadIdx.x == 0) ws.mats[id] = q;
     const int t0 = w * NTHR + threadIdx.x, ts = nw * NTHR;
-    for (int t = t0; t < q.batch * q.ntiles_sym; t += ts) ws.map_sym[q.sym0 + t] = id;
-    for (int t = t0; t < q.batch * q.tm * q.tn; t += ts) ws.map_rect[q.rect0 + t] = id;
+    for (int t = t0; t < q.nsym; t += ts) ws.map_sym[q.sym0 + t] = id;
+    for (int t = t0; t < q.nrect; t += ts) ws.map_rect[q.rect0 + t] = id;
     const int np_ = q.batch * ((q.mp + 63) / 64) * ((q.np + 63) / 64);
     for (int t = t0; t < np_; t += ts) ws.map_prep[q.prep0 + t] = id;
-    const int b = w / q.parts, part = w - b * q.parts;
-    const int64_t n = (int64_t)q.rows * q.cols, per = (n + q.parts - 1) / q.parts;
-    const int64_t e0 = part * per, e1 = e0 + per < n ? e0 + per : n;
-    const double s = q.dtype == DINO_F32
-                         ? row_range_sq<float>((const float*)q.in + b * q.in_batch, q.in_ld, q.cols, e0, e1)
-                         : row_range_sq<bf16>((const bf16*)q.in + b * q.in_batch, q.in_ld, q.cols, e0, e1);
+    const int b = w / q.parts, part = w - b * q.parts, per = (q.rows + q.parts - 1) / q.parts;
+    const int r0 = part * per, r1 = min(q.rows, r0 + per);
+    const double s = q.dtype == DINO_F32 ? rows_sq<float>(q.in, b * q.in_batch, q.in_ld, q.cols, r0, r1)
+                                         : rows_sq<bf16>(q.in, b * q.in_batch, q.in_ld, q.cols, r0, r1);
     const double tot = block_sum_f64(s, red);
     if (threadIdx.x == 0) ws.parts[q.part0 + w] = tot;
 }
@@ -152,198 +155,309 @@ __global__ __launch_bounds__(NTHR) void ortho_prep_kernel(const Ws ws, double ep
 
 struct GemmArgs {
     Ws ws;
-    int src, split, split_next;      // X buffer read, operands are pairs, the next step's operands are pairs
+    int src, split_next;             // X buffer read; the next step's operands are pairs
     float c0, c1;                    // epilogue: c0 * (elementwise operand) + c1 * product
 };
 
 DEVI int fsw(int x) { return (4 - (x & 3)) & 3; }
-DEVI int tkey(int row) { return 2 * ((row & 3) | (((row >> 3) & 1) << 2)); }
 template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// 128 x 128 tile of a product per workgroup (2 x 2 waves of 64 x 64).
+// T x T tile of a product per workgroup of eight waves (2 x 4, each T/2 x T/4).
 //   GRAM    A = X X^T             rows of X against rows of X; tiles on and above the diagonal, written twice
 //   POLY    B = b A + c A A       A symmetric: rows against rows again
 //   UPDATE  X' = a X + B X        rows of B against COLUMNS of X (transposing LDS reads)
 //   FINAL   the last UPDATE: into the caller's matrix as bf16
-// Operands go global -> LDS by DMA in a ring of S stages of 32 along the contraction; split operands are three passes
-// (hi hi, hi lo, lo hi) of one stream of stages.
+// Operands go global -> LDS by DMA in a ring of stages of 32 along the contraction; with SPLIT a stage holds the hi and lo
+// parts of both and feeds three products (hi hi, hi lo, lo hi): 3 products for 2 loads.  The path from L2 to the CUs
+// bounds these products (about 10 TB/s: T operations a byte), hence the large tiles and the shared split stages.
+// The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
+// multiplies.  Waves 4..7 (B) run one phase behind waves 0..3 (A); stage s is read in phases 2s (A) and 2s + 1 (B), its
+// slot is refilled from phase 2s + 2 on.
 enum { GRAM, POLY, UPDATE, FINAL };
-template <int MODE> __global__ __launch_bounds__(NTHR, 2) void ortho_gemm_kernel(const GemmArgs ga) {
+template <int T, bool SPLIT> struct Cfg {
+    static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
+    static constexpr int OPB = T * BK * 2, STAGE = (SPLIT ? 4 : 2) * OPB;
+    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : T == 192 ? (SPLIT ? 3 : 5) : (SPLIT ? 2 : 4);
+    static constexpr int ND = T / 64;                               // DMAs a wave, stage and part (hi / lo)
+    static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
+    static constexpr int LDT = SUBM + 4, LDN = SUBN + 4;            // rows of its image in LDS (elements), by column / row
+    static constexpr int IMG = (LDT * SUBN > LDN * SUBM ? LDT * SUBN : LDN * SUBM) * 2;
+    static constexpr int SMEM = S * STAGE > 8 * IMG ? S * STAGE : 8 * IMG;
+};
+// chunk permutation of a [32][T] stage: the eight rows that half a wave's transposing read touches lie in different banks
+template <int T> DEVI int tkey(int row) {
+    return T == 192 ? 2 * (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) : 2 * ((row & 3) | (((row >> 3) & 1) << 2));
+}
+
+DEVI unsigned pack2(float a, float b, bool to_bf16) {
+    if (to_bf16) {
+        const bf16x2 v = {(bf16)a, (bf16)b};
+        return __builtin_bit_cast(unsigned, v);
+    }
+    typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {(f16)a, (f16)b};
+    return __builtin_bit_cast(unsigned, v);
+}
+
+template <int MODE, int T, bool SPLIT>
+__global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const GemmArgs ga) {
 #if defined(__HIP_DEVICE_COMPILE__)
+    typedef Cfg<T, SPLIT> C;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, NP = SPLIT ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave >> 1, wn = wave & 1, i = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 2, wn = wave & 3, i = lane & 15, g = lane >> 4;
+    const bool late = wave >= 4;
     const int bid = xcd_remap(blockIdx.x, gridDim.x);
     const Ws& ws = ga.ws;
     const int id = SYM ? ws.map_sym[bid] : ws.map_rect[bid];
     const Mat& q = ws.mats[id];
     const int mp = q.mp, np = q.np;
+    const int tm = (mp + T - 1) / T, tn = (np + T - 1) / T;
     int t = bid - (SYM ? q.sym0 : q.rect0);
-    const int per = SYM ? q.ntiles_sym : q.tm * q.tn;
+    const int per = SYM ? tm * (tm + 1) / 2 : tm * tn;
     const int b = t / per;
     t -= b * per;
     int ti, tj;
     if (SYM) {
         ti = 0;
-        while (t >= q.tm - ti) { t -= q.tm - ti; ++ti; }
+        while (t >= tm - ti) { t -= tm - ti; ++ti; }
         tj = ti + t;
     } else {
-        tj = t / q.tm;               // the tiles of one column panel follow each other: it stays in L2
-        ti = t - tj * q.tm;
+        tj = t / tm;                 // the tiles of one column panel follow each other: it stays in L2
+        ti = t - tj * tm;
     }
-    const int m0 = ti * TILE, n0 = tj * TILE;
+    const int m0 = ti * T, n0 = tj * T;
     const int64_t xo = q.xoff + (int64_t)b * mp * np, ao = q.aoff + (int64_t)b * mp * mp;
-    const int ldp = MODE == GRAM ? np : mp, ldq = MODE == GRAM ? np : MODE == POLY ? mp : np;
-    const int K = MODE == GRAM ? np : mp;
-    const f16* P[2];
-    const f16* Q[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        P[h] = MODE == GRAM ? ws.x[ga.src][h] + xo : MODE == POLY ? ws.a[h] + ao : ws.b[h] + ao;
-        Q[h] = MODE == POLY ? ws.a[h] + ao : ws.x[ga.src][h] + xo;
-    }
-    const int pbytes = mp * ldp * 2, qbytes = mp * ldq * 2;
+    const int ldp = MODE == GRAM ? np : mp, ldq = MODE == POLY ? mp : np;
+    const int total = (MODE == GRAM ? np : mp) / BK;
+    const float e1 = ws.exps[q.mat0 + b], e2 = e1 * e1;
 
-    // ---- stages: 32 columns of 128 rows of P ([row][4 chunks of 16 B]), and of Q either the same or, for UPDATE, 32 rows
-    // of 128 columns ([k][16 chunks]); chunks are permuted by a key of the row so that neither kind of read meets
-    // itself in a bank.  Rows and columns behind the matrix read zeros or neighbours: only their own results, which
-    // are not stored, see them.
-    const int wv = __builtin_amdgcn_readfirstlane(wave);
-    int voP[2], voQ[2];
+    // ---- stages: 32 columns of T rows of P ([row][4 chunks of 16 B]), and of Q either the same or, for UPDATE, 32 rows
+    // of T columns ([k][T / 8 chunks]); chunks are permuted by a key of the row so that no read meets itself in a bank.
+    // Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not stored, see
+    // them.  A wave moves pieces wave, wave + 8, ... of 1 KB: first P's, then Q's.
+    __amdgpu_buffer_rsrc_t rsP[NP], rsQ[NP];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int L = tid + NTHR * u;
-        const int r = L >> 2, c = L & 3;
-        voP[u] = (r * ldp + ((c ^ fsw(r >> 2)) << 3)) * 2;
-        if (SYM) voQ[u] = (r * ldq + ((c ^ fsw(r >> 4)) << 3)) * 2;
-        else {
-            const int kr = L >> 4, kc = L & 15;
-            voQ[u] = (kr * ldq + ((kc ^ tkey(kr)) << 3)) * 2;
+    for (int h = 0; h < NP; ++h) {
+        const f16* P = MODE == GRAM ? ws.x[ga.src][h] + xo : MODE == POLY ? ws.a[h] + ao : ws.b[h] + ao;
+        const f16* Q = MODE == POLY ? ws.a[h] + ao : ws.x[ga.src][h] + xo;
+        rsP[h] = __builtin_amdgcn_make_buffer_rsrc((void*)P, 0, mp * ldp * 2, 0x00020000);
+        rsQ[h] = __builtin_amdgcn_make_buffer_rsrc((void*)Q, 0, mp * ldq * 2, 0x00020000);
+    }
+    int vo[ND];
+#pragma unroll
+    for (int u = 0; u < ND; ++u) {
+        const int d = wave + 8 * u;
+        const bool isP = d < T / 16;
+        const int L = (isP ? d : d - T / 16) * 64 + lane;
+        if (isP || SYM) {
+            const int r = L >> 2, c = L & 3;
+            vo[u] = (r * (isP ? ldp : ldq) + ((c ^ fsw(r >> 2)) << 3)) * 2;
+        } else {
+            const int r = L / (T / 8), c = L - r * (T / 8);
+            vo[u] = (r * ldq + ((c ^ tkey<T>(r)) << 3)) * 2;
         }
     }
-    const int nk = K / BK, nseg = ga.split ? 3 : 1, total = nk * nseg;
-    int iseg = 0, ik = 0, islot = 0;
-    __amdgpu_buffer_rsrc_t rsP = __builtin_amdgcn_make_buffer_rsrc((void*)P[0], 0, pbytes, 0x00020000);
-    __amdgpu_buffer_rsrc_t rsQ = __builtin_amdgcn_make_buffer_rsrc((void*)Q[0], 0, qbytes, 0x00020000);
+    int inext = 0, islot = 0;
     auto issue = [&]() {
-        const int sa = islot * STAGE + wv * 1024;
-        const int k = ik * BK;
-        const int soP = (m0 * ldp + k) * 2;
-        const int soQ = SYM ? (n0 * ldq + k) * 2 : (k * ldq + n0) * 2;
+        if (inext < total) {
+            const int k = inext * BK;
+            const int soP = (m0 * ldp + k) * 2, soQ = SYM ? (n0 * ldq + k) * 2 : (k * ldq + n0) * 2;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsP, (lptr_t)(smem + sa + u * 4096), 16, voP[u], soP, 0, 0);
+            for (int h = 0; h < NP; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsQ, (lptr_t)(smem + sa + OPB + u * 4096), 16, voQ[u], soQ, 0, 0);
+                for (int u = 0; u < ND; ++u) {
+                    const int d = wave + 8 * u;
+                    const bool isP = d < T / 16;
+                    const int at = islot * C::STAGE + h * 2 * C::OPB + d * 1024;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(isP ? rsP[h] : rsQ[h], (lptr_t)(smem + at), 16, vo[u],
+                                                             isP ? soP : soQ, 0, 0);
+                }
+        }
+        ++inext;
         islot = islot + 1 == S ? 0 : islot + 1;
-        if (++ik == nk) {
-            ik = 0;
-            ++iseg;                                   // 0: hi hi, 1: hi lo, 2: lo hi
-            rsP = __builtin_amdgcn_make_buffer_rsrc((void*)P[iseg == 2], 0, pbytes, 0x00020000);
-            rsQ = __builtin_amdgcn_make_buffer_rsrc((void*)Q[iseg == 1], 0, qbytes, 0x00020000);
+    };
+    auto landed = [&](int s) {       // my DMAs of stage s are done (inext: stages requested)
+        const int younger = min(inext, total) - 1 - s;
+        if (younger >= S - 1) wait_vmcnt<NP * ND * (S - 1)>();
+        else if (S > 2 && younger == S - 2) wait_vmcnt<NP * ND * (S - 2)>();
+        else if (S > 3 && younger == S - 3) wait_vmcnt<NP * ND * (S - 3)>();
+        else wait_vmcnt<0>();
+    };
+
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int a = 0; a < MI; ++a)
+#pragma unroll
+        for (int c = 0; c < NI; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int rp = wm * C::SUBM + i, offP = rp * 64 + ((g ^ fsw(rp >> 2)) << 4);
+    const int rq = wn * C::SUBN + i, offQ = C::OPB + rq * 64 + ((g ^ fsw(rq >> 2)) << 4);
+    int offT[NI];
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+        const int row = 8 * g + (i >> 2), ch = (wn * C::SUBN + ni * 16) / 8 + ((i & 3) >> 1);
+        offT[ni] = C::OPB + row * (2 * T) + ((ch ^ tkey<T>(row)) << 4) + (i & 1) * 8;
+    }
+    u32x4 fp[NP][MI], fq[NP][NI];
+    auto read = [&](const char* st) {
+#pragma unroll
+        for (int h = 0; h < NP; ++h) {
+            const char* sh = st + h * 2 * C::OPB;
+#pragma unroll
+            for (int x = 0; x < NI; ++x) {
+                if (SYM) fq[h][x] = *(const u32x4*)(sh + offQ + x * 1024);
+                else {
+                    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x])));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x] + 8 * T)));
+                    fq[h][x] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(sh + offP + x * 1024);
         }
     };
-    int issued = 0;
+    auto multiply = [&]() {
+        auto mm = [&](int hp, int hq) {
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s)
-        if (issued < total) { issue(); ++issued; }
-
-    f32x4 acc[4][4];
+            for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int ra0 = wm * 64 + i, rb0 = wn * 64 + 16 * (i >> 2) + (i & 3);
-    const int offP = ra0 * 64 + ((g ^ fsw(ra0 >> 2)) << 4);
-    const int offQ = OPB + rb0 * 64 + ((g ^ fsw(rb0 >> 4)) << 4);
-    int offT[4];
-#pragma unroll
-    for (int ni = 0; ni < 4; ++ni) {
-        const int row = 8 * g + (i >> 2), ch = (wn * 64 + ni * 16) / 8 + ((i & 3) >> 1);
-        offT[ni] = OPB + row * 256 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
-    }
-
-    int cslot = 0;
-    for (int s = 0; s < total; ++s) {
-        if (total - 1 - s >= S - 2) wait_vmcnt<4 * (S - 2)>();
-        else wait_vmcnt<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (issued < total) { issue(); ++issued; }
-        const char* st = smem + cslot * STAGE;
-        u32x4 fp[4], fq[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            if (SYM) fq[x] = *(const u32x4*)(st + offQ + x * 256);
-            else {
-                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st + offT[x])));
-                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(st + offT[x] + 1024)));
-                fq[x] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-            }
+                for (int ni = 0; ni < NI; ++ni)
+                    acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(f16x8, fq[hq][ni]), __builtin_bit_cast(f16x8, fp[hp][mi]), acc[mi][ni], 0, 0, 0);
+        };
+        if (SPLIT) {
+            mm(NP - 1, 0);
+            mm(0, NP - 1);
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) fp[x] = *(const u32x4*)(st + offP + x * 1024);
-#pragma unroll
-        for (int mi = 0; mi < 4; ++mi)
-#pragma unroll
-            for (int ni = 0; ni < 4; ++ni)
-                acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fq[ni]),
-                                                                     __builtin_bit_cast(f16x8, fp[mi]), acc[mi][ni], 0, 0, 0);
-        cslot = cslot + 1 == S ? 0 : cslot + 1;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // before a wave may refill this slot
+        mm(0, 0);
+    };
+    auto phase = [&]() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
+
+    for (int s = 0; s < S - 1; ++s) issue();
+    landed(0);
+    phase();                                                   // phase 0 begins
+    if (late) {
+        issue();
+        phase();
+    }
+    int slot = 0;
+    for (int s = 0; s < total; ++s) {
+        if (!late) issue();                                    // stage s + S - 1, into the slot that s - 1 has left
+        read(smem + slot * C::STAGE);
+        slot = slot + 1 == S ? 0 : slot + 1;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (late) landed(s + 1);
+        phase();
+        if (late) issue();
+        multiply();
+        if (!late) landed(s + 1);
+        if (!late || s + 1 < total) phase();
     }
 
-    // the matrix's own exponent: products of two (A) or three (B X) stored operands carry 2^2e too much
-    const float e1 = ws.exps[q.mat0 + b], e2 = e1 * e1;
+    // ---- epilogue.  Lane (i, g) holds columns 16 ni + 4 g + r of row 16 mi + i of its wave's part.
+    // The matrix's own exponent: products of two (A) or three (B X) stored operands carry 2^2e too much.
     const float c1 = MODE == GRAM ? ga.c1 : MODE == FINAL ? ga.c1 * e2 * e1 : ga.c1 * e2;
     const float c0 = MODE == FINAL ? ga.c0 * e1 : ga.c0;
-    // ---- epilogue: lane holds four consecutive columns of row m per fragment
+    const int wm0 = m0 + wm * C::SUBM, wn0 = n0 + wn * C::SUBN;
+    const int nend = SYM ? mp : np;
 #pragma unroll
-    for (int mi = 0; mi < 4; ++mi) {
-        const int m = m0 + wm * 64 + mi * 16 + i;
-        if (m >= mp) continue;
+    for (int mi = 0; mi < MI; ++mi) {
+        const int m = wm0 + mi * 16 + i;
 #pragma unroll
-        for (int ni = 0; ni < 4; ++ni) {
-            const int n = n0 + wn * 64 + (SYM ? 16 * g + 4 * ni : 16 * ni + 4 * g);
-            if (n >= (SYM ? mp : np)) continue;
-            float v[4];
+        for (int ni = 0; ni < NI; ++ni) {
+            const int n = wn0 + 16 * ni + 4 * g;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = c1 * acc[mi][ni][r];
-            if (MODE != GRAM) {
+            for (int r = 0; r < 4; ++r) acc[mi][ni][r] *= c1;
+            if (MODE != GRAM && m < mp && n < nend) {
                 const int64_t at = MODE == POLY ? ao + (int64_t)m * mp + n : xo + (int64_t)m * np + n;
                 const f16* eh = MODE == POLY ? ws.a[0] : ws.x[ga.src][0];
                 const f16* el = MODE == POLY ? ws.a[1] : ws.x[ga.src][1];
                 const f16x4 h = *(const f16x4*)(eh + at);
                 f16x4 l{};
-                if (ga.split) l = *(const f16x4*)(el + at);
+                if (SPLIT) l = *(const f16x4*)(el + at);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = fmaf(c0, (float)h[r] + (float)l[r], v[r]);
-            }
-            if (SYM) {
-                f16* oh = (MODE == GRAM ? ws.a[0] : ws.b[0]) + ao;
-                f16* ol = (MODE == GRAM ? ws.a[1] : ws.b[1]) + ao;
-                split_store(oh + (int64_t)m * mp + n, ga.split ? ol + (int64_t)m * mp + n : nullptr, v);
-                if (ti != tj) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const f16 h = (f16)v[r];
-                        oh[(int64_t)(n + r) * mp + m] = h;
-                        if (ga.split) ol[(int64_t)(n + r) * mp + m] = (f16)(v[r] - (float)h);
-                    }
-                }
-            } else if (MODE == UPDATE) {
-                const int64_t at = xo + (int64_t)m * np + n;
-                split_store(ws.x[ga.src ^ 1][0] + at, ga.split_next ? ws.x[ga.src ^ 1][1] + at : nullptr, v);
-            } else {
-                if (m >= q.m) continue;
-                bf16* out = (bf16*)q.out + b * q.out_batch;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < q.n) out[q.tall ? (int64_t)(n + r) * q.out_ld + m : (int64_t)m * q.out_ld + n + r] = (bf16)v[r];
+                for (int r = 0; r < 4; ++r) acc[mi][ni][r] = fmaf(c0, (float)h[r] + (float)l[r], acc[mi][ni][r]);
             }
         }
+    }
+    // Results leave through an image of the wave's part in LDS (all stages are done with; a wave reads only what it wrote),
+    // by rows or by columns, so that every store covers whole rows of the destination.
+    char* img = smem + wave * C::IMG;
+    constexpr bool TOBF = MODE == FINAL;
+    auto emit = [&](auto by_col_c, void* dst, int64_t ld, int rows, int cols, bool aligned) {
+        constexpr bool COL = decltype(by_col_c)::value;       // destination rows are columns of the tile
+        constexpr int LDI = COL ? C::LDT : C::LDN;            // elements a row of the image
+        constexpr int NR = COL ? C::SUBN : C::SUBM, NC = COL ? C::SUBM : C::SUBN;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                const f32x4 v = acc[mi][ni];
+                if (!COL) {
+                    const u32x2 w = {pack2(v[0], v[1], TOBF), pack2(v[2], v[3], TOBF)};
+                    *(u32x2*)(img + ((mi * 16 + i) * LDI + ni * 16 + 4 * g) * 2) = w;
+                } else {
+                    // lanes i and i ^ 1 (rows m, m + 1) trade: the even one gets columns r = 0, 1 of both, the odd one 2, 3
+                    const bool odd = i & 1;
+                    const float x0 = dpp_mov<0xB1>(odd ? v[0] : v[2]), x1 = dpp_mov<0xB1>(odd ? v[1] : v[3]);
+                    const int c = ni * 16 + 4 * g + (odd ? 2 : 0), m = mi * 16 + (i & ~1);
+                    *(unsigned*)(img + (c * LDI + m) * 2) = odd ? pack2(x0, v[2], TOBF) : pack2(v[0], x0, TOBF);
+                    *(unsigned*)(img + ((c + 1) * LDI + m) * 2) = odd ? pack2(x1, v[3], TOBF) : pack2(v[1], x1, TOBF);
+                }
+            }
+        const int r0 = COL ? wn0 : wm0, q0 = COL ? wm0 : wn0;  // destination of the image's origin
+        constexpr int LPR = NC / 4;                            // lanes a row, four elements each
+        for (int e = lane; e < NR * LPR; e += 64) {
+            const int r = e / LPR, c = (e - r * LPR) * 4;
+            const u32x2 w = *(const u32x2*)(img + (r * LDI + c) * 2);
+            if (r0 + r >= rows || q0 + c >= cols) continue;
+            uint16_t* o = (uint16_t*)dst + (int64_t)(r0 + r) * ld + q0 + c;
+            if (aligned && q0 + c + 4 <= cols) *(u32x2*)o = w;
+            else {
+                const unsigned x[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (q0 + c + k < cols) o[k] = (uint16_t)x[k];
+            }
+        }
+    };
+    auto take_hi = [&]() {           // what the fp16 of the image has left of the values
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[mi][ni][r] -= (float)(f16)acc[mi][ni][r];
+    };
+    if (SYM) {
+        f16** o = MODE == GRAM ? (f16**)ws.a : (f16**)ws.b;
+        emit(std::false_type{}, o[0] + ao, mp, mp, mp, true);
+        if (ti != tj) emit(std::true_type{}, o[0] + ao, mp, mp, mp, true);
+        if (SPLIT) {
+            take_hi();
+            emit(std::false_type{}, o[1] + ao, mp, mp, mp, true);
+            if (ti != tj) emit(std::true_type{}, o[1] + ao, mp, mp, mp, true);
+        }
+    } else if (MODE == UPDATE) {
+        emit(std::false_type{}, ws.x[ga.src ^ 1][0] + xo, np, mp, np, true);
+        if (SPLIT && ga.split_next) {
+            take_hi();
+            emit(std::false_type{}, ws.x[ga.src ^ 1][1] + xo, np, mp, np, true);
+        }
+    } else {
+        bf16* out = (bf16*)q.out + b * q.out_batch;
+        const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 7) == 0;
+        if (q.tall) emit(std::true_type{}, out, q.out_ld, q.n, q.m, al);
+        else emit(std::false_type{}, out, q.out_ld, q.m, q.n, al);
     }
 #endif
 }
@@ -354,6 +468,7 @@ int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 struct Layout {
     int64_t bytes, mats, maps[3], parts, exps, x, a;      // byte offsets; x / a: first region, xbytes / abytes apart
     int64_t xbytes, abytes, ntile[3];
+    int tile[2];                                    // of the symmetric products, of the update
 };
 
 int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
@@ -372,21 +487,53 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         q.mp = (int)up(q.m, 32);
         q.np = (int)up(q.n, 32);
         if ((int64_t)q.mp * q.np * 2 >= (1ll << 31)) return DINO_ERR_TOO_LARGE;
-        q.tm = (q.mp + TILE - 1) / TILE;
-        q.tn = (q.np + TILE - 1) / TILE;
-        q.ntiles_sym = q.tm * (q.tm + 1) / 2;
         int64_t p = ((int64_t)q.m * q.n + 16383) / 16384;
-        q.parts = (int)(p > 256 ? 256 : p);
-        q.part0 = (int)parts; q.mat0 = (int)nmat; q.xoff = xo; q.aoff = ao; q.sym0 = (int)sym; q.rect0 = (int)rect; q.prep0 = (int)prep;
+        if (p > 256) p = 256;
+        q.parts = (int)(p > q.rows ? q.rows : p);
+        q.part0 = (int)parts; q.mat0 = (int)nmat; q.xoff = xo; q.aoff = ao; q.prep0 = (int)prep;
         parts += (int64_t)s.batch * q.parts;
         nmat += s.batch;
         xo += (int64_t)s.batch * q.mp * q.np;
         ao += (int64_t)s.batch * q.mp * q.mp;
-        sym += (int64_t)s.batch * q.ntiles_sym;
-        rect += (int64_t)s.batch * q.tm * q.tn;
         prep += (int64_t)s.batch * ((q.mp + 63) / 64) * ((q.np + 63) / 64);
         if (prep >= (1 << 24) || parts >= (1 << 24)) return DINO_ERR_TOO_LARGE;    // 256 threads each, < 2^32 a launch
         if (out) out[i] = q;
+    }
+    // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
+    // the CUs, a tile costing its area over the rate that the path from L2 allows (T operations a byte, and no
+    // more than about two thirds of the matrix pipes).
+    for (int kind = 0; kind < 2; ++kind) {
+        double best = 0;
+        const int sizes[3] = {256, 192, 128};
+        for (int z = 0; z < 3; ++z) {
+            const int T = sizes[z];
+            double work = 0, tiles = 0;
+            for (int i = 0; i < count; ++i) {
+                int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
+                int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
+                const double tm = (double)((m + T - 1) / T), tn = (double)((n + T - 1) / T);
+                const double k = kind ? tm * tn * items[i].batch : tm * (tm + 1) / 2 * items[i].batch;
+                tiles += k;
+                work += k * (double)(kind ? m : n + m);
+            }
+            if (tiles == 0) tiles = 1;
+            const double cost = work / tiles * ceil(tiles / (T == 128 ? 512.0 : 256.0)) * T * T / (T == 256 ? 1.0 : T == 192 ? 0.8 : 0.35);
+            if (z == 0 || cost < best) { best = cost; L.tile[kind] = T; }
+        }
+        static const char* force[2] = {getenv("OT_SYM"), getenv("OT_RECT")};
+        if (force[kind]) L.tile[kind] = atoi(force[kind]);
+    }
+    for (int i = 0; i < count; ++i) {
+        int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
+        int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
+        const int64_t ts = (m + L.tile[0] - 1) / L.tile[0], tm = (m + L.tile[1] - 1) / L.tile[1], tn = (n + L.tile[1] - 1) / L.tile[1];
+        const int64_t ns = items[i].batch * (ts * (ts + 1) / 2), nr = items[i].batch * tm * tn;
+        if (out) {
+            out[i].sym0 = (int)sym; out[i].rect0 = (int)rect;
+            out[i].nsym = (int)ns; out[i].nrect = (int)nr;
+        }
+        sym += ns;
+        rect += nr;
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at = up(at + bytes, 256); return r; };
@@ -413,10 +560,18 @@ void poly_bounds(const float* c, double top, double& px, double& qx) {
     }
 }
 
-template <int MODE> int launch_gemm(const GemmArgs& ga, int64_t grid, hipStream_t st) {
-    constexpr int smem = S * STAGE;
-    hipLaunchKernelGGL((ortho_gemm_kernel<MODE>), dim3((unsigned)grid), dim3(NTHR), smem, st, ga);
+template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, int64_t grid, hipStream_t st) {
+    constexpr int smem = Cfg<T, SPLIT>::SMEM;
+    static const hipError_t set = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>,
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (set != hipSuccess) return (int)set;
+    hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3((unsigned)grid), dim3(512), smem, st, ga);
     return dino_launch_status();
+}
+template <int MODE> int launch_gemm(const GemmArgs& ga, int T, bool split, int64_t grid, hipStream_t st) {
+    if (T == 256) return split ? launch_as<MODE, 256, true>(ga, grid, st) : launch_as<MODE, 256, false>(ga, grid, st);
+    if (T == 192) return split ? launch_as<MODE, 192, true>(ga, grid, st) : launch_as<MODE, 192, false>(ga, grid, st);
+    return split ? launch_as<MODE, 128, true>(ga, grid, st) : launch_as<MODE, 128, false>(ga, grid, st);
 }
 
 }  // namespace
@@ -496,17 +651,18 @@ extern "C" int dino_ortho(const dino_ortho_item* items, int count, int steps, co
     rc = dino_launch_status();
     for (int s = 0; s < steps && rc == DINO_OK; ++s) {
         const float* c = coeffs + 3 * s;
-        GemmArgs ga{ws, s & 1, split(s), split(s + 1), 0.f, (float)(sa[s] / ((double)SX * SX))};
-        rc = launch_gemm<GRAM>(ga, L.ntile[0], st);
+        GemmArgs ga{ws, s & 1, split(s + 1), 0.f, (float)(sa[s] / ((double)SX * SX))};
+        rc = launch_gemm<GRAM>(ga, L.tile[0], split(s), L.ntile[0], st);
         if (rc != DINO_OK) break;
         ga.c0 = (float)(c[1] * sb[s] / sa[s]);
         ga.c1 = (float)(c[2] * sb[s] / (sa[s] * sa[s]));
-        rc = launch_gemm<POLY>(ga, L.ntile[0], st);
+        rc = launch_gemm<POLY>(ga, L.tile[0], split(s), L.ntile[0], st);
         if (rc != DINO_OK) break;
         const double o = s + 1 == steps ? 1.0 / SX : 1.0;
         ga.c0 = (float)(c[0] * o);
         ga.c1 = (float)(o / sb[s]);
-        rc = s + 1 == steps ? launch_gemm<FINAL>(ga, L.ntile[1], st) : launch_gemm<UPDATE>(ga, L.ntile[1], st);
+        rc = s + 1 == steps ? launch_gemm<FINAL>(ga, L.tile[1], split(s), L.ntile[1], st)
+                            : launch_gemm<UPDATE>(ga, L.tile[1], split(s), L.ntile[1], st);
     }
     return rc;
 }
