@@ -47,6 +47,7 @@ struct Setup {
     int wg0[ITEMS + 1];                         // first workgroup of each item
     int count, first;                           // items here, index of the first
 };
+// X, A, B lie as panels of 32 columns: element (r, c) of a matrix of mp rows at ((c / 32) mp + r) 32 + c % 32.
 struct Ws {                                     // regions of the workspace
     Mat* mats;
     int *map_sym, *map_rect, *map_prep;         // tile -> item
@@ -146,7 +147,7 @@ __global__ __launch_bounds__(NTHR) void ortho_prep_kernel(const Ws ws, double ep
     for (int r = r0; r < 64; r += 4) {
         if (m0 + r >= q.mp || n0 + c >= q.np) continue;
         const float v = q.tall ? tile[c][r] : tile[r][c];
-        const int64_t at = (int64_t)(m0 + r) * q.np + n0 + c;
+        const int64_t at = ((int64_t)((n0 + c) >> 5) * q.mp + m0 + r) * 32 + ((n0 + c) & 31);
         const f16 h = (f16)v;
         xh[at] = h;
         if (lo) xl[at] = (f16)(v - (float)h);
@@ -184,10 +185,9 @@ template <int T, bool SPLIT> struct Cfg {
     static constexpr int IMG = (LDT * SUBN > LDN * SUBM ? LDT * SUBN : LDN * SUBM) * 2;
     static constexpr int SMEM = S * STAGE > 8 * IMG ? S * STAGE : 8 * IMG;
 };
-// chunk permutation of a [32][T] stage: the eight rows that half a wave's transposing read touches lie in different banks
-template <int T> DEVI int tkey(int row) {
-    return T == 192 ? 2 * (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) : 2 * ((row & 3) | (((row >> 3) & 1) << 2));
-}
+// chunk permutation of a [32 rows][4 chunks] panel: the eight rows (8 apart in two groups of four) that half a wave's
+// transposing read touches lie in different banks
+DEVI int tkey(int row) { return 2 * ((row >> 3) & 1); }
 
 DEVI unsigned pack2(float a, float b, bool to_bf16) {
     if (to_bf16) {
@@ -231,41 +231,41 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     }
     const int m0 = ti * T, n0 = tj * T;
     const int64_t xo = q.xoff + (int64_t)b * mp * np, ao = q.aoff + (int64_t)b * mp * mp;
-    const int ldp = MODE == GRAM ? np : mp, ldq = MODE == POLY ? mp : np;
     const int total = (MODE == GRAM ? np : mp) / BK;
     const float e1 = ws.exps[q.mat0 + b], e2 = e1 * e1;
 
     // ---- stages: 32 columns of T rows of P ([row][4 chunks of 16 B]), and of Q either the same or, for UPDATE, 32 rows
-    // of T columns ([k][T / 8 chunks]); chunks are permuted by a key of the row so that no read meets itself in a bank.
-    // Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not stored, see
-    // them.  A wave moves pieces wave, wave + 8, ... of 1 KB: first P's, then Q's.
+    // of T columns (T / 32 panels of [32 rows][4 chunks]).  The operands lie in memory as panels of 32 columns, so every
+    // DMA of a wave moves 1 KB in one piece.  Chunks are permuted by a key of the row so that no read meets itself
+    // in a bank.  Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not
+    // stored, see them.  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
     __amdgpu_buffer_rsrc_t rsP[NP], rsQ[NP];
 #pragma unroll
     for (int h = 0; h < NP; ++h) {
         const f16* P = MODE == GRAM ? ws.x[ga.src][h] + xo : MODE == POLY ? ws.a[h] + ao : ws.b[h] + ao;
         const f16* Q = MODE == POLY ? ws.a[h] + ao : ws.x[ga.src][h] + xo;
-        rsP[h] = __builtin_amdgcn_make_buffer_rsrc((void*)P, 0, mp * ldp * 2, 0x00020000);
-        rsQ[h] = __builtin_amdgcn_make_buffer_rsrc((void*)Q, 0, mp * ldq * 2, 0x00020000);
+        rsP[h] = __builtin_amdgcn_make_buffer_rsrc((void*)P, 0, mp * (MODE == GRAM ? np : mp) * 2, 0x00020000);
+        rsQ[h] = __builtin_amdgcn_make_buffer_rsrc((void*)Q, 0, mp * (MODE == POLY ? mp : np) * 2, 0x00020000);
     }
     int vo[ND];
 #pragma unroll
     for (int u = 0; u < ND; ++u) {
         const int d = wave + 8 * u;
         const bool isP = d < T / 16;
-        const int L = (isP ? d : d - T / 16) * 64 + lane;
+        const int e = isP ? d : d - T / 16;
         if (isP || SYM) {
-            const int r = L >> 2, c = L & 3;
-            vo[u] = (r * (isP ? ldp : ldq) + ((c ^ fsw(r >> 2)) << 3)) * 2;
+            const int r = e * 16 + (lane >> 2);
+            vo[u] = r * 64 + (((lane & 3) ^ fsw(r >> 2)) << 4);
         } else {
-            const int r = L / (T / 8), c = L - r * (T / 8);
-            vo[u] = (r * ldq + ((c ^ tkey<T>(r)) << 3)) * 2;
+            const int r = (e & 1) * 16 + (lane >> 2);
+            vo[u] = (e >> 1) * mp * 64 + r * 64 + (((lane & 3) ^ tkey(r)) << 4);
         }
     }
     int inext = 0, islot = 0;
     auto issue = [&]() {
         if (inext < total) {
-            const int k = inext * BK;
-            const int soP = (m0 * ldp + k) * 2, soQ = SYM ? (n0 * ldq + k) * 2 : (k * ldq + n0) * 2;
+            const int soP = (inext * mp + m0) * 64;
+            const int soQ = SYM ? (inext * mp + n0) * 64 : ((n0 >> 5) * mp + inext * 32) * 64;
 #pragma unroll
             for (int h = 0; h < NP; ++h)
 #pragma unroll
@@ -298,8 +298,8 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     int offT[NI];
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
-        const int row = 8 * g + (i >> 2), ch = (wn * C::SUBN + ni * 16) / 8 + ((i & 3) >> 1);
-        offT[ni] = C::OPB + row * (2 * T) + ((ch ^ tkey<T>(row)) << 4) + (i & 1) * 8;
+        const int row = 8 * g + (i >> 2), col = wn * C::SUBN + ni * 16, ch = (col & 31) / 8 + ((i & 3) >> 1);
+        offT[ni] = C::OPB + (col >> 5) * 2048 + row * 64 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
     }
     u32x4 fp[NP][MI], fq[NP][NI];
     auto read = [&](const char* st) {
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                 if (SYM) fq[h][x] = *(const u32x4*)(sh + offQ + x * 1024);
                 else {
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x])));
-                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x] + 8 * T)));
+                    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x] + 256)));
                     fq[h][x] = u32x4{lo[0], lo[1], hi[0], hi[1]};
                 }
             }
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[mi][ni][r] *= c1;
             if (MODE != GRAM && m < mp && n < nend) {
-                const int64_t at = MODE == POLY ? ao + (int64_t)m * mp + n : xo + (int64_t)m * np + n;
+                const int64_t at = (MODE == POLY ? ao : xo) + ((int64_t)(n >> 5) * mp + m) * 32 + (n & 31);
                 const f16* eh = MODE == POLY ? ws.a[0] : ws.x[ga.src][0];
                 const f16* el = MODE == POLY ? ws.a[1] : ws.x[ga.src][1];
                 const f16x4 h = *(const f16x4*)(eh + at);
@@ -389,8 +389,22 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
             }
         }
     }
-    // Results leave through an image of the wave's part in LDS (all stages are done with; a wave reads only what it wrote),
-    // by rows or by columns, so that every store covers whole rows of the destination.
+    // fp16 results go to panels: 32 bytes of 16 rows a store
+    auto put = [&](f16* dst) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+            const int m = wm0 + mi * 16 + i;
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                const int n = wn0 + 16 * ni + 4 * g;
+                const f32x4 v = acc[mi][ni];
+                if (m < mp && n < nend)
+                    *(u32x2*)(dst + ((int64_t)(n >> 5) * mp + m) * 32 + (n & 31)) = u32x2{pack2(v[0], v[1], false), pack2(v[2], v[3], false)};
+            }
+        }
+    };
+    // ... mirrored ones, and the caller's bf16, through an image of the wave's part in LDS (all stages are done with; a
+    // wave reads only what it wrote), by rows or by columns, so that every store covers rows of the destination.
     char* img = smem + wave * C::IMG;
     constexpr bool TOBF = MODE == FINAL;
     auto emit = [&](auto by_col_c, void* dst, int64_t ld, int rows, int cols, bool aligned) {
@@ -417,16 +431,22 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         const int r0 = COL ? wn0 : wm0, q0 = COL ? wm0 : wn0;  // destination of the image's origin
         constexpr int LPR = NC / 4;                            // lanes a row, four elements each
         for (int e = lane; e < NR * LPR; e += 64) {
-            const int r = e / LPR, c = (e - r * LPR) * 4;
+            int r = e / LPR, c = (e - r * LPR) * 4;
+            if (!TOBF) {                                       // panels: 64 bytes of one row after the other
+                const int pan = e / (8 * NR), f = e - pan * (8 * NR);
+                r = f >> 3;
+                c = pan * 32 + (f & 7) * 4;
+            }
             const u32x2 w = *(const u32x2*)(img + (r * LDI + c) * 2);
-            if (r0 + r >= rows || q0 + c >= cols) continue;
-            uint16_t* o = (uint16_t*)dst + (int64_t)(r0 + r) * ld + q0 + c;
-            if (aligned && q0 + c + 4 <= cols) *(u32x2*)o = w;
+            const int dr = r0 + r, dc = q0 + c;
+            if (dr >= rows || dc >= cols) continue;
+            uint16_t* o = (uint16_t*)dst + (TOBF ? dr * ld + dc : ((int64_t)(dc >> 5) * ld + dr) * 32 + (dc & 31));
+            if (aligned && dc + 4 <= cols) *(u32x2*)o = w;
             else {
                 const unsigned x[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (q0 + c + k < cols) o[k] = (uint16_t)x[k];
+                    if (dc + k < cols) o[k] = (uint16_t)x[k];
             }
         }
     };
@@ -439,19 +459,19 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                 for (int r = 0; r < 4; ++r) acc[mi][ni][r] -= (float)(f16)acc[mi][ni][r];
     };
     if (SYM) {
-        f16** o = MODE == GRAM ? (f16**)ws.a : (f16**)ws.b;
-        emit(std::false_type{}, o[0] + ao, mp, mp, mp, true);
+        f16* const* o = MODE == GRAM ? ws.a : ws.b;
+        put(o[0] + ao);
         if (ti != tj) emit(std::true_type{}, o[0] + ao, mp, mp, mp, true);
         if (SPLIT) {
             take_hi();
-            emit(std::false_type{}, o[1] + ao, mp, mp, mp, true);
+            put(o[1] + ao);
             if (ti != tj) emit(std::true_type{}, o[1] + ao, mp, mp, mp, true);
         }
     } else if (MODE == UPDATE) {
-        emit(std::false_type{}, ws.x[ga.src ^ 1][0] + xo, np, mp, np, true);
+        put(ws.x[ga.src ^ 1][0] + xo);
         if (SPLIT && ga.split_next) {
             take_hi();
-            emit(std::false_type{}, ws.x[ga.src ^ 1][1] + xo, np, mp, np, true);
+            put(ws.x[ga.src ^ 1][1] + xo);
         }
     } else {
         bf16* out = (bf16*)q.out + b * q.out_batch;
