@@ -15,6 +15,7 @@
 #include <math.h>
 #include <stdlib.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -40,8 +41,24 @@ struct Mat {
     int rows, cols, batch, dtype;
     int tall, m, n, mp, np;                     // m <= n; mp, np: padded to 32 (zeros)
     int parts, part0, mat0;                     // partial sums of the norm: per matrix, first index; first matrix
-    int sym0, rect0, prep0, nsym, nrect;        // first global tile of each kind; tiles of the whole item
+    int preps;                                  // 64 x 64 tiles that a workgroup of the preparing kernel takes
+    int sym0, rect0, prep0;                     // first tile of each kind
 };
+// One tile of a product: everything a workgroup needs to start on it, in one load.
+struct Tile {
+    int64_t xo, ao;                             // the matrix in the X and A / B regions (elements)
+    int mp, np, m0, n0, item, mat;              // mat: index within the item
+    int all, pad;                               // index of the matrix over all items
+};
+// (read as constant memory, that is through scalar loads: it was written by an earlier launch)
+DEVI Tile load_tile(const Tile* p) {
+    typedef const __attribute__((address_space(4))) u32x4* cptr_t;
+    struct { u32x4 w[3]; } t;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) t.w[i] = ((cptr_t)(uintptr_t)p)[i];
+    return __builtin_bit_cast(Tile, t);
+}
+DEVI float load_const(const float* p) { return *(const __attribute__((address_space(4))) float*)(uintptr_t)p; }
 struct Setup {
     Mat it[ITEMS];
     int wg0[ITEMS + 1];                         // first workgroup of each item
@@ -50,9 +67,11 @@ struct Setup {
 // X, A, B lie as panels of 32 columns: element (r, c) of a matrix of mp rows at ((c / 32) mp + r) 32 + c % 32.
 struct Ws {                                     // regions of the workspace
     Mat* mats;
-    int *map_sym, *map_rect, *map_prep;         // tile -> item
+    Tile *sym, *rect;                           // tiles of the symmetric products / of the update
+    int* map_prep;                              // workgroup of the preparing kernel -> item
     double* parts;
-    float* exps;                                // per matrix: 2^-e
+    float* exps;                                // 2^-e of each matrix
+    int tsym, trect;                            // tile sizes
     f16 *x[2][2], *a[2], *b[2];                 // [buffer][hi / lo]
 };
 
@@ -92,8 +111,10 @@ template <typename T> DEVI double rows_sq(const void* in, int64_t at, int64_t ld
     return rows_sq<T, 1>(p, ld, cols, r0, r1);
 }
 
-// Partial sums of squares (fp64: neither 1e-30 nor 1e30 leaves the range), and the item table with the tile -> item maps
-// that the following launches read.
+DEVI int prep_groups(const Mat& q) { return (((q.mp + 63) / 64) * ((q.np + 63) / 64) + q.preps - 1) / q.preps; }
+
+// Partial sums of squares (fp64: neither 1e-30 nor 1e30 leaves the range), and the tables that the
+// following launches read: items, the map of the preparing kernel, the products' tiles.
 __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const Ws ws) {
     __shared__ double red[4];
     int i = 0;
@@ -102,10 +123,28 @@ __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const 
     const int w = blockIdx.x - su.wg0[i], nw = su.wg0[i + 1] - su.wg0[i], id = su.first + i;
     if (w == 0 && threadIdx.x == 0) ws.mats[id] = q;
     const int t0 = w * NTHR + threadIdx.x, ts = nw * NTHR;
-    for (int t = t0; t < q.nsym; t += ts) ws.map_sym[q.sym0 + t] = id;
-    for (int t = t0; t < q.nrect; t += ts) ws.map_rect[q.rect0 + t] = id;
-    const int np_ = q.batch * ((q.mp + 63) / 64) * ((q.np + 63) / 64);
+    const int np_ = q.batch * prep_groups(q);
     for (int t = t0; t < np_; t += ts) ws.map_prep[q.prep0 + t] = id;
+    // the tiles of the products
+    const int sm = (q.mp + ws.tsym - 1) / ws.tsym, ns = sm * (sm + 1) / 2;
+    const int rm = (q.mp + ws.trect - 1) / ws.trect, nr = rm * ((q.np + ws.trect - 1) / ws.trect);
+    for (int t = t0; t < q.batch * (ns + nr); t += ts) {
+        const bool sym = t < q.batch * ns;
+        const int u = sym ? t : t - q.batch * ns, mat = u / (sym ? ns : nr);
+        int k = u - mat * (sym ? ns : nr);
+        Tile d{q.xoff + (int64_t)mat * q.mp * q.np, q.aoff + (int64_t)mat * q.mp * q.mp, q.mp, q.np, 0, 0, id, mat, q.mat0 + mat, 0};
+        if (sym) {
+            int ti = 0;
+            while (k >= sm - ti) { k -= sm - ti; ++ti; }
+            d.m0 = ti * ws.tsym;
+            d.n0 = (ti + k) * ws.tsym;
+            ws.sym[q.sym0 + u] = d;
+        } else {                             // one column panel after the other: it stays in L2
+            d.m0 = (k % rm) * ws.trect;
+            d.n0 = (k / rm) * ws.trect;
+            ws.rect[q.rect0 + u] = d;
+        }
+    }
     const int b = w / q.parts, part = w - b * q.parts, per = (q.rows + q.parts - 1) / q.parts;
     const int r0 = part * per, r1 = min(q.rows, r0 + per);
     const double s = q.dtype == DINO_F32 ? rows_sq<float>(q.in, b * q.in_batch, q.in_ld, q.cols, r0, r1)
@@ -114,83 +153,138 @@ __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const 
     if (threadIdx.x == 0) ws.parts[q.part0 + w] = tot;
 }
 
-// X0 = U * SX / (|U| + eps) as hi + lo, shorter side in front, padding cleared: 64 x 64 tiles through LDS where U is tall.
+// X0 = U * SX 2^e / (|U| + eps) as hi + lo in panels, shorter side in front, padding cleared; 64 x 64 elements at a time,
+// through LDS where U is tall.  VEC: U's rows start at multiples of four elements.
+template <typename T, bool VEC> DEVI void prep_tiles(const Mat& q, const T* u, f16* xh, f16* xl, int t0, int t1, float scale, float (&tile)[64][66]) {
+    const int tn = (q.np + 63) / 64, c4 = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
+    for (int t = t0; t < t1; ++t) {
+        const int m0 = (t / tn) * 64, n0 = (t % tn) * 64;
+        float v[4][4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {            // row ur, columns uc .. uc + 3 of U
+            const int ur = (q.tall ? n0 : m0) + r0 + 16 * p, uc = (q.tall ? m0 : n0) + c4;
+            const T* x = u + ur * q.in_ld + uc;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[p][k] = 0.f;
+            if (ur < q.rows) {
+                if (VEC && uc + 4 <= q.cols) load4<T>(x, v[p]);
+                else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (uc + k < q.cols) v[p][k] = to_f32<T>(x[k]);
+                }
+            }
+        }
+        if (q.tall) {
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tile[r0 + 16 * p][c4 + k] = v[p][k];
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[p][k] = tile[c4 + k][r0 + 16 * p];
+        }
+        const int n = n0 + c4;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int m = m0 + r0 + 16 * p;
+            if (m >= q.mp || n >= q.np) continue;
+            const int64_t at = ((int64_t)(n >> 5) * q.mp + m) * 32 + (n & 31);
+            f16x4 h, l;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float x = v[p][k] * scale;
+                h[k] = (f16)x;
+                l[k] = (f16)(x - (float)h[k]);
+            }
+            *(f16x4*)(xh + at) = h;
+            if (xl) *(f16x4*)(xl + at) = l;
+        }
+    }
+}
 __global__ __launch_bounds__(NTHR) void ortho_prep_kernel(const Ws ws, double eps, double gain, int lo) {
     __shared__ double red[4];
-    __shared__ float tile[64][65];
+    __shared__ float tile[64][66];
     const int id = ws.map_prep[blockIdx.x];
     const Mat& q = ws.mats[id];
-    const int tm = (q.mp + 63) / 64, tn = (q.np + 63) / 64;
-    int t = blockIdx.x - q.prep0;
-    const int b = t / (tm * tn);
-    t -= b * tm * tn;
-    const int m0 = (t / tn) * 64, n0 = (t % tn) * 64;
+    const int per = prep_groups(q), w = blockIdx.x - q.prep0, b = w / per, part = w - b * per;
     double s = 0;
     for (int p = threadIdx.x; p < q.parts; p += NTHR) s += ws.parts[q.part0 + b * q.parts + p];
     const double norm = sqrt(block_sum_f64(s, red)), end = gain * (norm / (norm + eps));
     const int e = end > 0.0 && end < 1.0 ? min(80, ilogb(1.0 / end)) : 0;
     const float scale = (float)(ldexp((double)SX, e) / (norm + eps));
-    if (t == 0 && threadIdx.x == 0) ws.exps[q.mat0 + b] = ldexpf(1.f, -e);
-    const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
-    for (int r = r0; r < 64; r += 4) {       // rows of U: m0.. of X, or n0.. where U is tall
-        const int ur = (q.tall ? n0 : m0) + r, uc = (q.tall ? m0 : n0) + c;
-        float v = 0.f;
-        if (ur < q.rows && uc < q.cols) {
-            const int64_t at = b * q.in_batch + ur * q.in_ld + uc;
-            v = (q.dtype == DINO_F32 ? ((const float*)q.in)[at] : (float)((const bf16*)q.in)[at]) * scale;
-        }
-        tile[r][c] = v;
-    }
-    __syncthreads();
-    f16* xh = ws.x[0][0] + q.xoff + (int64_t)b * q.mp * q.np;
-    f16* xl = ws.x[0][1] + q.xoff + (int64_t)b * q.mp * q.np;
-    for (int r = r0; r < 64; r += 4) {
-        if (m0 + r >= q.mp || n0 + c >= q.np) continue;
-        const float v = q.tall ? tile[c][r] : tile[r][c];
-        const int64_t at = ((int64_t)((n0 + c) >> 5) * q.mp + m0 + r) * 32 + ((n0 + c) & 31);
-        const f16 h = (f16)v;
-        xh[at] = h;
-        if (lo) xl[at] = (f16)(v - (float)h);
+    if (part == 0 && threadIdx.x == 0) ws.exps[q.mat0 + b] = ldexpf(1.f, -e);
+    const int nt = ((q.mp + 63) / 64) * ((q.np + 63) / 64), t0 = part * q.preps, t1 = min(nt, t0 + q.preps);
+    const int64_t xo = q.xoff + (int64_t)b * q.mp * q.np;
+    f16 *xh = ws.x[0][0] + xo, *xl = lo ? ws.x[0][1] + xo : nullptr;
+    if (q.dtype == DINO_F32) {
+        const float* u = (const float*)q.in + b * q.in_batch;
+        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 4)) & 15) == 0) prep_tiles<float, true>(q, u, xh, xl, t0, t1, scale, tile);
+        else prep_tiles<float, false>(q, u, xh, xl, t0, t1, scale, tile);
+    } else {
+        const bf16* u = (const bf16*)q.in + b * q.in_batch;
+        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 2)) & 7) == 0) prep_tiles<bf16, true>(q, u, xh, xl, t0, t1, scale, tile);
+        else prep_tiles<bf16, false>(q, u, xh, xl, t0, t1, scale, tile);
     }
 }
 
 struct GemmArgs {
     Ws ws;
-    int src, split_next;             // X buffer read; the next step's operands are pairs
-    float c0, c1;                    // epilogue: c0 * (elementwise operand) + c1 * product
+    int src, split_next, ntiles;     // X buffer read; the next step's operands are pairs; tiles of this launch
+    float c0, c1, ca;                // epilogue: c0 * (elementwise operand) + c1 * product, + ca on the diagonal
 };
 
 DEVI int fsw(int x) { return (4 - (x & 3)) & 3; }
 template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// T x T tile of a product per workgroup of eight waves (2 x 4, each T/2 x T/4).
-//   GRAM    A = X X^T             rows of X against rows of X; tiles on and above the diagonal, written twice
-//   POLY    B = b A + c A A       A symmetric: rows against rows again
-//   UPDATE  X' = a X + B X        rows of B against COLUMNS of X (transposing LDS reads)
+// T x T tiles of a product, a workgroup of eight waves (2 x 4, each T/2 x T/4) walking its share of them.
+//   GRAM    A = X X^T               rows of X against rows of X; tiles on and above the diagonal, written twice
+//   POLY    B = a I + b A + c A A   A symmetric: rows against rows again
+//   UPDATE  X' = B X                rows of B against COLUMNS of X (transposing LDS reads)
 //   FINAL   the last UPDATE: into the caller's matrix as bf16
-// Operands go global -> LDS by DMA in a ring of stages of 32 along the contraction; with SPLIT a stage holds the hi and lo
-// parts of both and feeds three products (hi hi, hi lo, lo hi): 3 products for 2 loads.  The path from L2 to the CUs
-// bounds these products (about 10 TB/s: T operations a byte), hence the large tiles and the shared split stages.
+// (a on B's diagonal instead of a X in the update: no second read of X.)
+// Operands go global -> LDS by DMA in a ring of S stages of 32 along the contraction, one stream of stages over all tiles of
+// the workgroup: the next tile's first stages are on their way while this one's results leave.  With SPLIT a stage
+// holds the hi and lo parts of both operands and feeds three products (hi hi, hi lo, lo hi): 3 products for 2 loads.  The
+// path from L2 to the CUs bounds these products (about 9.4 TB/s: T / 2 operations a byte), hence the large tiles.
 // The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
-// multiplies.  Waves 4..7 (B) run one phase behind waves 0..3 (A); stage s is read in phases 2s (A) and 2s + 1 (B), its
-// slot is refilled from phase 2s + 2 on.
+// multiplies.  Waves 4..7 ("late") run one phase behind waves 0..3: stage s is read in phases 2s and 2s + 1, its slot is
+// refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
     static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
     static constexpr int OPB = T * BK * 2, STAGE = (SPLIT ? 4 : 2) * OPB;
-    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : T == 192 ? (SPLIT ? 3 : 5) : (SPLIT ? 2 : 4);
+    static constexpr int S = SPLIT ? 2 : 4;                         // 128 KB (T = 256), 64 KB (T = 128)
     static constexpr int ND = T / 64;                               // DMAs a wave, stage and part (hi / lo)
     static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
-    static constexpr int LDT = SUBM + 4, LDN = SUBN + 4;            // rows of its image in LDS (elements), by column / row
-    static constexpr int IMG = (LDT * SUBN > LDN * SUBM ? LDT * SUBN : LDN * SUBM) * 2;
-    static constexpr int SMEM = S * STAGE > 8 * IMG ? S * STAGE : 8 * IMG;
+    static constexpr int IMG = 16 * SUBM * 2;                       // image of 16 columns of it
+    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 160 KB / 80 KB: one / two workgroups a CU
 };
+// The DMA is written in assembly: behind the builtin the compiler waits for ALL requests before every transposing LDS
+// read, which may alias what is being filled for all it knows.  It has no register result; the waits are landed()'s.
+// M0 is written nowhere else.
+DEVI u32x4 rsrc(const void* p, int bytes) {
+    const uint64_t a = (uint64_t)p;
+    u32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+    r[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);         // offsets past the end are dropped
+    r[3] = 0x00020000;
+    return r;
+}
+DEVI void dma16(unsigned lds, int voff, const u32x4& rs, int soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(lds), "v"(voff), "s"(rs), "s"(soff) : "memory");
+}
 // chunk permutation of a [32 rows][4 chunks] panel: the eight rows (8 apart in two groups of four) that half a wave's
 // transposing read touches lie in different banks
 DEVI int tkey(int row) { return 2 * ((row >> 3) & 1); }
 
-DEVI unsigned pack2(float a, float b, bool to_bf16) {
-    if (to_bf16) {
+template <bool TOBF> DEVI unsigned pack2(float a, float b) {
+    if (TOBF) {
         const bf16x2 v = {(bf16)a, (bf16)b};
         return __builtin_bit_cast(unsigned, v);
     }
@@ -210,89 +304,81 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, i = lane & 15, g = lane >> 4;
     const bool late = wave >= 4;
-    const int bid = xcd_remap(blockIdx.x, gridDim.x);
     const Ws& ws = ga.ws;
-    const int id = SYM ? ws.map_sym[bid] : ws.map_rect[bid];
-    const Mat& q = ws.mats[id];
-    const int mp = q.mp, np = q.np;
-    const int tm = (mp + T - 1) / T, tn = (np + T - 1) / T;
-    int t = bid - (SYM ? q.sym0 : q.rect0);
-    const int per = SYM ? tm * (tm + 1) / 2 : tm * tn;
-    const int b = t / per;
-    t -= b * per;
-    int ti, tj;
-    if (SYM) {
-        ti = 0;
-        while (t >= tm - ti) { t -= tm - ti; ++ti; }
-        tj = ti + t;
-    } else {
-        tj = t / tm;                 // the tiles of one column panel follow each other: it stays in L2
-        ti = t - tj * tm;
-    }
-    const int m0 = ti * T, n0 = tj * T;
-    const int64_t xo = q.xoff + (int64_t)b * mp * np, ao = q.aoff + (int64_t)b * mp * mp;
-    const int total = (MODE == GRAM ? np : mp) / BK;
-    const float e1 = ws.exps[q.mat0 + b], e2 = e1 * e1;
+    const Tile* tiles = SYM ? ws.sym : ws.rect;
+    // workgroup -> tiles b, b + G, ...: in every round an XCD has neighbouring tiles
+    const int G = gridDim.x, b0 = xcd_remap(blockIdx.x, G);
+    const int nmine = (ga.ntiles - b0 + G - 1) / G;
 
     // ---- stages: 32 columns of T rows of P ([row][4 chunks of 16 B]), and of Q either the same or, for UPDATE, 32 rows
     // of T columns (T / 32 panels of [32 rows][4 chunks]).  The operands lie in memory as panels of 32 columns, so every
     // DMA of a wave moves 1 KB in one piece.  Chunks are permuted by a key of the row so that no read meets itself
     // in a bank.  Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not
     // stored, see them.  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
-    __amdgpu_buffer_rsrc_t rsP[NP], rsQ[NP];
-#pragma unroll
-    for (int h = 0; h < NP; ++h) {
-        const f16* P = MODE == GRAM ? ws.x[ga.src][h] + xo : MODE == POLY ? ws.a[h] + ao : ws.b[h] + ao;
-        const f16* Q = MODE == POLY ? ws.a[h] + ao : ws.x[ga.src][h] + xo;
-        rsP[h] = __builtin_amdgcn_make_buffer_rsrc((void*)P, 0, mp * (MODE == GRAM ? np : mp) * 2, 0x00020000);
-        rsQ[h] = __builtin_amdgcn_make_buffer_rsrc((void*)Q, 0, mp * (MODE == POLY ? mp : np) * 2, 0x00020000);
-    }
     int vo[ND];
 #pragma unroll
     for (int u = 0; u < ND; ++u) {
-        const int d = wave + 8 * u;
-        const bool isP = d < T / 16;
-        const int e = isP ? d : d - T / 16;
-        if (isP || SYM) {
-            const int r = e * 16 + (lane >> 2);
-            vo[u] = r * 64 + (((lane & 3) ^ fsw(r >> 2)) << 4);
-        } else {
-            const int r = (e & 1) * 16 + (lane >> 2);
-            vo[u] = (e >> 1) * mp * 64 + r * 64 + (((lane & 3) ^ tkey(r)) << 4);
-        }
+        const bool isP = u < ND / 2;
+        const int e = wave + 8 * u - (isP ? 0 : T / 16);
+        const int r = (isP || SYM ? e * 16 : (e & 1) * 16) + (lane >> 2);
+        vo[u] = r * 64 + (((lane & 3) ^ (isP || SYM ? fsw(r >> 2) : tkey(r))) << 4);
     }
-    int inext = 0, islot = 0;
+    u32x4 rsP[NP], rsQ[NP];
+    const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
+    int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, islot = 0, issued = 0;
+    Tile tn = load_tile(tiles + b0);                       // the tile after the one being requested
+    auto open = [&]() {                        // start requesting tile tn
+        imp = tn.mp;
+        im0 = tn.m0;
+        in0 = tn.n0;
+        itotal = (MODE == GRAM ? tn.np : tn.mp) / BK;
+#pragma unroll
+        for (int h = 0; h < NP; ++h) {
+            const f16* P = MODE == GRAM ? ws.x[ga.src][h] + tn.xo : MODE == POLY ? ws.a[h] + tn.ao : ws.b[h] + tn.ao;
+            const f16* Q = MODE == POLY ? ws.a[h] + tn.ao : ws.x[ga.src][h] + tn.xo;
+            rsP[h] = rsrc(P, tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
+            rsQ[h] = rsrc(Q, tn.mp * (MODE == POLY ? tn.mp : tn.np) * 2);
+        }
+        if (ji + 1 < nmine) tn = load_tile(tiles + b0 + (ji + 1) * G);
+    };
+    open();
     auto issue = [&]() {
-        if (inext < total) {
-            const int soP = (inext * mp + m0) * 64;
-            const int soQ = SYM ? (inext * mp + n0) * 64 : ((n0 >> 5) * mp + inext * 32) * 64;
+        if (ji < nmine) {
+            const int soP = (ik * imp + im0) * 64;
+            const int soQ = SYM ? (ik * imp + in0) * 64 : ((in0 >> 5) * imp + ik * 32) * 64;
 #pragma unroll
             for (int h = 0; h < NP; ++h)
 #pragma unroll
                 for (int u = 0; u < ND; ++u) {
+                    const bool isP = u < ND / 2;
                     const int d = wave + 8 * u;
-                    const bool isP = d < T / 16;
-                    const int at = islot * C::STAGE + h * 2 * C::OPB + d * 1024;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(isP ? rsP[h] : rsQ[h], (lptr_t)(smem + at), 16, vo[u],
-                                                             isP ? soP : soQ, 0, 0);
+                    const int so = isP ? soP : SYM ? soQ : soQ + ((d - T / 16) >> 1) * imp * 64;
+                    dma16(lds0 + islot * C::STAGE + h * 2 * C::OPB + d * 1024, vo[u], isP ? rsP[h] : rsQ[h], so);
                 }
+            ++issued;
+            if (++ik == itotal) {
+                ik = 0;
+                if (++ji < nmine) open();
+            }
         }
-        ++inext;
         islot = islot + 1 == S ? 0 : islot + 1;
     };
-    auto landed = [&](int s) {       // my DMAs of stage s are done (inext: stages requested)
-        const int younger = min(inext, total) - 1 - s;
-        if (younger >= S - 1) wait_vmcnt<NP * ND * (S - 1)>();
-        else if (S > 2 && younger == S - 2) wait_vmcnt<NP * ND * (S - 2)>();
-        else if (S > 3 && younger == S - 3) wait_vmcnt<NP * ND * (S - 3)>();
+    auto landed = [&](int s) {       // my DMAs of stage s are done
+        const int younger = issued - 1 - s;
+        if (S == 4 && younger >= 3) wait_vmcnt<NP * ND * 3>();
+        else if (S == 4 && younger == 2) wait_vmcnt<NP * ND * 2>();
+        else if (younger >= 1) wait_vmcnt<NP * ND>();
         else wait_vmcnt<0>();
     };
 
     f32x4 acc[MI][NI];
+    auto clear = [&]() {
 #pragma unroll
-    for (int a = 0; a < MI; ++a)
+        for (int a = 0; a < MI; ++a)
 #pragma unroll
-        for (int c = 0; c < NI; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < NI; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    clear();
     const int rp = wm * C::SUBM + i, offP = rp * 64 + ((g ^ fsw(rp >> 2)) << 4);
     const int rq = wn * C::SUBN + i, offQ = C::OPB + rq * 64 + ((g ^ fsw(rq >> 2)) << 4);
     int offT[NI];
@@ -302,7 +388,10 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         offT[ni] = C::OPB + (col >> 5) * 2048 + row * 64 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
     }
     u32x4 fp[NP][MI], fq[NP][NI];
-    auto read = [&](const char* st) {
+    int slot = 0;
+    auto read = [&]() {
+        const char* st = smem + slot * C::STAGE;
+        slot = slot + 1 == S ? 0 : slot + 1;
 #pragma unroll
         for (int h = 0; h < NP; ++h) {
             const char* sh = st + h * 2 * C::OPB;
@@ -318,6 +407,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
             for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(sh + offP + x * 1024);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     auto multiply = [&]() {
         auto mm = [&](int hp, int hq) {
@@ -342,142 +432,200 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         asm volatile("" ::: "memory");
     };
 
+    // ---- results of a tile.  Lane (i, g) holds columns 16 ni + 4 g + r of row 16 mi + i of its wave's part.
+    char* img = smem + S * C::STAGE + wave * C::IMG;
+    auto finish = [&](const Tile& d, float e1) {
+        const int mp = d.mp, np = d.np;
+        // the matrix's own exponent: products of two stored X (A) carry 2^2e, of two A's 2^4e too much; B is kept without
+        const float e2 = e1 * e1;
+        const float c0 = ga.c0 * e2, c1 = MODE == POLY ? ga.c1 * e2 * e2 : MODE == FINAL ? ga.c1 * e1 : ga.c1;
+        const int wm0 = d.m0 + wm * C::SUBM, wn0 = d.n0 + wn * C::SUBN;
+        const int nend = SYM ? mp : np;
+        // where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 32, so a
+        // fragment is inside as a whole or outside as a whole)
+        const int vlane = i * 64 + g * 8;
+        auto upart = [&](int ni) {           // (+ 1024 mi)
+            const int n = wn0 + 16 * ni;
+            return ((n >> 5) * mp + wm0) * 64 + (n & 31) * 2;
+        };
+        if (MODE == POLY) {
+            // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads a neighbour or
+            // zero and is not stored)
+            __amdgpu_buffer_rsrc_t rs[NP];
+#pragma unroll
+            for (int h = 0; h < NP; ++h) rs[h] = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a[h] + d.ao), 0, mp * mp * 2, 0x00020000);
+            constexpr int PART = MI / (SPLIT ? 4 : 2);
+#pragma unroll
+            for (int q = 0; q < MI; q += PART) {
+                f16x4 el[NP][PART][NI];
+#pragma unroll
+                for (int h = 0; h < NP; ++h)
+#pragma unroll
+                    for (int mi = 0; mi < PART; ++mi)
+#pragma unroll
+                        for (int ni = 0; ni < NI; ++ni)
+                            el[h][mi][ni] = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rs[h], vlane + (q + mi) * 1024, upart(ni), 0));
+#pragma unroll
+                for (int mi = 0; mi < PART; ++mi)
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float x = (float)el[0][mi][ni][r];
+                            if (SPLIT) x += (float)el[NP - 1][mi][ni][r];
+                            acc[q + mi][ni][r] = fmaf(c0, x, acc[q + mi][ni][r] * c1);
+                        }
+            }
+            if (d.m0 == d.n0) {
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (wm0 + mi * 16 + i == wn0 + 16 * ni + 4 * g + r) acc[mi][ni][r] += ga.ca;
+            }
+        } else {
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[mi][ni][r] *= c1;
+        }
+        // fp16 results go to panels: 32 bytes of 16 rows a store
+        auto put = [&](f16* dst) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)dst, 0, mp * nend * 2, 0x00020000);
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+                if (wn0 + 16 * ni >= nend) continue;
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) {
+                    if (wm0 + 16 * mi >= mp) continue;
+                    const f32x4 v = acc[mi][ni];
+                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])}, rs,
+                                                          vlane + mi * 1024, upart(ni), 0);
+                }
+            }
+        };
+        // ... by columns (a mirrored tile, a tall matrix of the caller's) through an image of 16 columns at a time in LDS, so
+        // that a store covers rows of the destination; a wave reads only what it wrote.
+        auto put_columns = [&](auto tobf_c, uint16_t* dst, int64_t ld, int rows, int cols, bool aligned) {
+            constexpr bool TOBF = decltype(tobf_c)::value;
+            constexpr int RB = C::SUBM * 2;
+            auto at = [&](int c, int m) { return c * RB + ((m * 2) ^ ((c >> 1 & (C::SUBM / 16 - 1)) << 5)); };
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) {
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) {
+                    // lanes i and i ^ 1 (rows m, m + 1) trade: the even one gets columns r = 0, 1 of both, the odd one 2, 3
+                    const f32x4 v = acc[mi][ni];
+                    const bool odd = i & 1;
+                    const float x0 = dpp_mov<0xB1>(odd ? v[0] : v[2]), x1 = dpp_mov<0xB1>(odd ? v[1] : v[3]);
+                    const int c = 4 * g + (odd ? 2 : 0), m = mi * 16 + (i & ~1);
+                    *(unsigned*)(img + at(c, m)) = odd ? pack2<TOBF>(x0, v[2]) : pack2<TOBF>(v[0], x0);
+                    *(unsigned*)(img + at(c + 1, m)) = odd ? pack2<TOBF>(x1, v[3]) : pack2<TOBF>(v[1], x1);
+                }
+                for (int e = lane; e < 4 * C::SUBM; e += 64) {
+                    // panels: 64 bytes of each of the 16 columns; else whole columns
+                    const int c = TOBF ? e / (C::SUBM / 4) : (e >> 3) & 15;
+                    const int m = TOBF ? (e - c * (C::SUBM / 4)) * 4 : (e >> 7) * 32 + (e & 7) * 4;
+                    const u32x2 w = *(const u32x2*)(img + at(c, m));
+                    const int dr = wn0 + ni * 16 + c, dc = wm0 + m;
+                    if (dr >= rows || dc >= cols) continue;
+                    uint16_t* o = dst + (TOBF ? dr * ld + dc : ((int64_t)(dc >> 5) * ld + dr) * 32 + (dc & 31));
+                    if (!TOBF || (aligned && dc + 4 <= cols)) *(u32x2*)o = w;
+                    else {
+                        const unsigned x[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (dc + k < cols) o[k] = (uint16_t)x[k];
+                    }
+                }
+            }
+        };
+        auto take_hi = [&]() {       // what the fp16 just written has left of the values
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[mi][ni][r] -= (float)(f16)acc[mi][ni][r];
+        };
+        if (SYM) {
+            f16* const* o = MODE == GRAM ? ws.a : ws.b;
+            put(o[0] + d.ao);
+            if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)(o[0] + d.ao), mp, mp, mp, true);
+            if (SPLIT) {
+                take_hi();
+                put(o[1] + d.ao);
+                if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)(o[1] + d.ao), mp, mp, mp, true);
+            }
+        } else if (MODE == UPDATE) {
+            put(ws.x[ga.src ^ 1][0] + d.xo);
+            if (SPLIT && ga.split_next) {
+                take_hi();
+                put(ws.x[ga.src ^ 1][1] + d.xo);
+            }
+        } else {
+            const Mat& q = ws.mats[d.item];
+            bf16* out = (bf16*)q.out + d.mat * q.out_batch;
+            const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 7) == 0;
+            if (q.tall) put_columns(std::true_type{}, (uint16_t*)out, q.out_ld, q.n, q.m, al);
+            else {
+#pragma unroll
+                for (int mi = 0; mi < MI; ++mi) {
+                    const int m = wm0 + mi * 16 + i;
+                    if (m >= q.m) continue;
+#pragma unroll
+                    for (int ni = 0; ni < NI; ++ni) {
+                        const int n = wn0 + 16 * ni + 4 * g;
+                        const f32x4 v = acc[mi][ni];
+                        bf16* o = out + m * q.out_ld + n;
+                        if (al && n + 4 <= q.n) *(u32x2*)o = u32x2{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])};
+                        else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (n + r < q.n) o[r] = (bf16)v[r];
+                        }
+                    }
+                }
+            }
+        }
+        clear();
+    };
+
+    // ---- the stream of stages.  Early waves read stage s in phase 2s and multiply in 2s + 1, late ones a phase later; a
+    // tile that ended with s is finished by both in phase 2s + 2, where stage s + S is requested into the slot of s.
     for (int s = 0; s < S - 1; ++s) issue();
+    Tile cur = load_tile(tiles + b0), nxt = load_tile(tiles + b0 + (nmine > 1 ? G : 0));
+    int total = (MODE == GRAM ? cur.np : cur.mp) / BK, j = 0, k = 0;
+    float e1 = load_const(ws.exps + cur.all);
     landed(0);
-    phase();                                                   // phase 0 begins
-    if (late) {
-        issue();
-        phase();
-    }
-    int slot = 0;
-    for (int s = 0; s < total; ++s) {
-        if (!late) issue();                                    // stage s + S - 1, into the slot that s - 1 has left
-        read(smem + slot * C::STAGE);
-        slot = slot + 1 == S ? 0 : slot + 1;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    phase();
+    issue();
+    if (late) phase();
+    for (int s = 0;; ++s) {
+        read();
         if (late) landed(s + 1);
         phase();
         if (late) issue();
         multiply();
-        if (!late) landed(s + 1);
-        if (!late || s + 1 < total) phase();
-    }
-
-    // ---- epilogue.  Lane (i, g) holds columns 16 ni + 4 g + r of row 16 mi + i of its wave's part.
-    // The matrix's own exponent: products of two (A) or three (B X) stored operands carry 2^2e too much.
-    const float c1 = MODE == GRAM ? ga.c1 : MODE == FINAL ? ga.c1 * e2 * e1 : ga.c1 * e2;
-    const float c0 = MODE == FINAL ? ga.c0 * e1 : ga.c0;
-    const int wm0 = m0 + wm * C::SUBM, wn0 = n0 + wn * C::SUBN;
-    const int nend = SYM ? mp : np;
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-        const int m = wm0 + mi * 16 + i;
-#pragma unroll
-        for (int ni = 0; ni < NI; ++ni) {
-            const int n = wn0 + 16 * ni + 4 * g;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[mi][ni][r] *= c1;
-            if (MODE != GRAM && m < mp && n < nend) {
-                const int64_t at = (MODE == POLY ? ao : xo) + ((int64_t)(n >> 5) * mp + m) * 32 + (n & 31);
-                const f16* eh = MODE == POLY ? ws.a[0] : ws.x[ga.src][0];
-                const f16* el = MODE == POLY ? ws.a[1] : ws.x[ga.src][1];
-                const f16x4 h = *(const f16x4*)(eh + at);
-                f16x4 l{};
-                if (SPLIT) l = *(const f16x4*)(el + at);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[mi][ni][r] = fmaf(c0, (float)h[r] + (float)l[r], acc[mi][ni][r]);
-            }
+        if (!late) {
+            landed(s + 1);
+            phase();
+            issue();
         }
-    }
-    // fp16 results go to panels: 32 bytes of 16 rows a store
-    auto put = [&](f16* dst) {
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-            const int m = wm0 + mi * 16 + i;
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-                const int n = wn0 + 16 * ni + 4 * g;
-                const f32x4 v = acc[mi][ni];
-                if (m < mp && n < nend)
-                    *(u32x2*)(dst + ((int64_t)(n >> 5) * mp + m) * 32 + (n & 31)) = u32x2{pack2(v[0], v[1], false), pack2(v[2], v[3], false)};
-            }
+        if (++k == total) {
+            finish(cur, e1);
+            if (++j == nmine) break;
+            cur = nxt;
+            e1 = load_const(ws.exps + cur.all);
+            if (j + 1 < nmine) nxt = load_tile(tiles + b0 + (j + 1) * G);
+            total = (MODE == GRAM ? cur.np : cur.mp) / BK;
+            k = 0;
         }
-    };
-    // ... mirrored ones, and the caller's bf16, through an image of the wave's part in LDS (all stages are done with; a
-    // wave reads only what it wrote), by rows or by columns, so that every store covers rows of the destination.
-    char* img = smem + wave * C::IMG;
-    constexpr bool TOBF = MODE == FINAL;
-    auto emit = [&](auto by_col_c, void* dst, int64_t ld, int rows, int cols, bool aligned) {
-        constexpr bool COL = decltype(by_col_c)::value;       // destination rows are columns of the tile
-        constexpr int LDI = COL ? C::LDT : C::LDN;            // elements a row of the image
-        constexpr int NR = COL ? C::SUBN : C::SUBM, NC = COL ? C::SUBM : C::SUBN;
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
-                const f32x4 v = acc[mi][ni];
-                if (!COL) {
-                    const u32x2 w = {pack2(v[0], v[1], TOBF), pack2(v[2], v[3], TOBF)};
-                    *(u32x2*)(img + ((mi * 16 + i) * LDI + ni * 16 + 4 * g) * 2) = w;
-                } else {
-                    // lanes i and i ^ 1 (rows m, m + 1) trade: the even one gets columns r = 0, 1 of both, the odd one 2, 3
-                    const bool odd = i & 1;
-                    const float x0 = dpp_mov<0xB1>(odd ? v[0] : v[2]), x1 = dpp_mov<0xB1>(odd ? v[1] : v[3]);
-                    const int c = ni * 16 + 4 * g + (odd ? 2 : 0), m = mi * 16 + (i & ~1);
-                    *(unsigned*)(img + (c * LDI + m) * 2) = odd ? pack2(x0, v[2], TOBF) : pack2(v[0], x0, TOBF);
-                    *(unsigned*)(img + ((c + 1) * LDI + m) * 2) = odd ? pack2(x1, v[3], TOBF) : pack2(v[1], x1, TOBF);
-                }
-            }
-        const int r0 = COL ? wn0 : wm0, q0 = COL ? wm0 : wn0;  // destination of the image's origin
-        constexpr int LPR = NC / 4;                            // lanes a row, four elements each
-        for (int e = lane; e < NR * LPR; e += 64) {
-            int r = e / LPR, c = (e - r * LPR) * 4;
-            if (!TOBF) {                                       // panels: 64 bytes of one row after the other
-                const int pan = e / (8 * NR), f = e - pan * (8 * NR);
-                r = f >> 3;
-                c = pan * 32 + (f & 7) * 4;
-            }
-            const u32x2 w = *(const u32x2*)(img + (r * LDI + c) * 2);
-            const int dr = r0 + r, dc = q0 + c;
-            if (dr >= rows || dc >= cols) continue;
-            uint16_t* o = (uint16_t*)dst + (TOBF ? dr * ld + dc : ((int64_t)(dc >> 5) * ld + dr) * 32 + (dc & 31));
-            if (aligned && dc + 4 <= cols) *(u32x2*)o = w;
-            else {
-                const unsigned x[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (dc + k < cols) o[k] = (uint16_t)x[k];
-            }
-        }
-    };
-    auto take_hi = [&]() {           // what the fp16 of the image has left of the values
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-            for (int ni = 0; ni < NI; ++ni)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[mi][ni][r] -= (float)(f16)acc[mi][ni][r];
-    };
-    if (SYM) {
-        f16* const* o = MODE == GRAM ? ws.a : ws.b;
-        put(o[0] + ao);
-        if (ti != tj) emit(std::true_type{}, o[0] + ao, mp, mp, mp, true);
-        if (SPLIT) {
-            take_hi();
-            put(o[1] + ao);
-            if (ti != tj) emit(std::true_type{}, o[1] + ao, mp, mp, mp, true);
-        }
-    } else if (MODE == UPDATE) {
-        put(ws.x[ga.src ^ 1][0] + xo);
-        if (SPLIT && ga.split_next) {
-            take_hi();
-            put(ws.x[ga.src ^ 1][1] + xo);
-        }
-    } else {
-        bf16* out = (bf16*)q.out + b * q.out_batch;
-        const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 7) == 0;
-        if (q.tall) emit(std::true_type{}, out, q.out_ld, q.n, q.m, al);
-        else emit(std::false_type{}, out, q.out_ld, q.m, q.n, al);
+        if (late) phase();
     }
 #endif
 }
@@ -486,7 +634,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 struct Layout {
-    int64_t bytes, mats, maps[3], parts, exps, x, a;      // byte offsets; x / a: first region, xbytes / abytes apart
+    int64_t bytes, mats, sym, rect, map, parts, exps, x, a;      // byte offsets; x / a: first region, xbytes / abytes apart
     int64_t xbytes, abytes, ntile[3];
     int tile[2];                                    // of the symmetric products, of the update
 };
@@ -510,56 +658,64 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         int64_t p = ((int64_t)q.m * q.n + 16383) / 16384;
         if (p > 256) p = 256;
         q.parts = (int)(p > q.rows ? q.rows : p);
-        q.part0 = (int)parts; q.mat0 = (int)nmat; q.xoff = xo; q.aoff = ao; q.prep0 = (int)prep;
+        const int64_t pt = (int64_t)((q.mp + 63) / 64) * ((q.np + 63) / 64);
+        q.preps = (int)(pt * s.batch > 16384 ? 8 : pt * s.batch > 4096 ? 2 : 1);
+        q.mat0 = (int)nmat;
+        q.part0 = (int)parts; q.xoff = xo; q.aoff = ao; q.prep0 = (int)prep;
         parts += (int64_t)s.batch * q.parts;
-        nmat += s.batch;
         xo += (int64_t)s.batch * q.mp * q.np;
         ao += (int64_t)s.batch * q.mp * q.mp;
-        prep += (int64_t)s.batch * ((q.mp + 63) / 64) * ((q.np + 63) / 64);
+        prep += (int64_t)s.batch * ((pt + q.preps - 1) / q.preps);
+        nmat += s.batch;
         if (prep >= (1 << 24) || parts >= (1 << 24)) return DINO_ERR_TOO_LARGE;    // 256 threads each, < 2^32 a launch
         if (out) out[i] = q;
     }
     // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
-    // the CUs, a tile costing its area over the rate that the path from L2 allows (T operations a byte, and no
-    // more than about two thirds of the matrix pipes).
+    // the CUs, a tile costing its operands' way from L2 (T a stage); of the smaller ones two share a CU, and what one
+    // starts and ends with overlaps the other: 0.65.
     for (int kind = 0; kind < 2; ++kind) {
         double best = 0;
-        const int sizes[3] = {256, 192, 128};
-        for (int z = 0; z < 3; ++z) {
-            const int T = sizes[z];
+        for (int T = 256; T >= 128; T /= 2) {
             double work = 0, tiles = 0;
             for (int i = 0; i < count; ++i) {
-                int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
-                int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
+                const int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
+                const int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
                 const double tm = (double)((m + T - 1) / T), tn = (double)((n + T - 1) / T);
                 const double k = kind ? tm * tn * items[i].batch : tm * (tm + 1) / 2 * items[i].batch;
                 tiles += k;
                 work += k * (double)(kind ? m : n + m);
             }
             if (tiles == 0) tiles = 1;
-            const double cost = work / tiles * ceil(tiles / (T == 128 ? 512.0 : 256.0)) * T * T / (T == 256 ? 1.0 : T == 192 ? 0.8 : 0.35);
-            if (z == 0 || cost < best) { best = cost; L.tile[kind] = T; }
+            const double cost = work / tiles * ceil(tiles / 256) * (T == 256 ? 256 : 83);
+            if (T == 256 || cost < best) { best = cost; L.tile[kind] = T; }
         }
         static const char* force[2] = {getenv("OT_SYM"), getenv("OT_RECT")};
         if (force[kind]) L.tile[kind] = atoi(force[kind]);
     }
-    for (int i = 0; i < count; ++i) {
-        int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
-        int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
-        const int64_t ts = (m + L.tile[0] - 1) / L.tile[0], tm = (m + L.tile[1] - 1) / L.tile[1], tn = (n + L.tile[1] - 1) / L.tile[1];
-        const int64_t ns = items[i].batch * (ts * (ts + 1) / 2), nr = items[i].batch * tm * tn;
-        if (out) {
-            out[i].sym0 = (int)sym; out[i].rect0 = (int)rect;
-            out[i].nsym = (int)ns; out[i].nrect = (int)nr;
+    // tiles with the longest contraction first: the last round then ends evenly
+    int* order = (int*)malloc(sizeof(int) * (size_t)(count + 1));
+    if (!order) return DINO_ERR_TOO_LARGE;
+    for (int i = 0; i < count; ++i) order[i] = i;
+    auto lo_side = [&](int i) { return items[i].rows < items[i].cols ? items[i].rows : items[i].cols; };
+    auto hi_side = [&](int i) { return items[i].rows < items[i].cols ? items[i].cols : items[i].rows; };
+    for (int kind = 0; kind < 2; ++kind) {
+        std::stable_sort(order, order + count, [&](int a, int b) { return kind ? lo_side(a) > lo_side(b) : hi_side(a) > hi_side(b); });
+        for (int o = 0; o < count; ++o) {
+            const int i = order[o], T = L.tile[kind];
+            const int64_t m = up(lo_side(i), 32), n = up(hi_side(i), 32), tm = (m + T - 1) / T;
+            int64_t& at = kind ? rect : sym;
+            if (out) (kind ? out[i].rect0 : out[i].sym0) = (int)at;
+            at += items[i].batch * (kind ? tm * ((n + T - 1) / T) : tm * (tm + 1) / 2);
         }
-        sym += ns;
-        rect += nr;
     }
+    free(order);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t r = at; at = up(at + bytes, 256); return r; };
     L.ntile[0] = sym; L.ntile[1] = rect; L.ntile[2] = prep;
     L.mats = take((int64_t)sizeof(Mat) * count);
-    for (int k = 0; k < 3; ++k) L.maps[k] = take(4 * L.ntile[k]);
+    L.sym = take((int64_t)sizeof(Tile) * sym);
+    L.rect = take((int64_t)sizeof(Tile) * rect);
+    L.map = take(4 * prep);
     L.parts = take(8 * parts);
     L.exps = take(4 * nmat);
     L.xbytes = up(2 * xo, 256);
@@ -570,28 +726,29 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
     return DINO_OK;
 }
 
-// largest |p(x)| and |b x^2 + c x^4| over singular values up to `top`
+// largest |p(x)| and |a + b x^2 + c x^4| over singular values up to `top`
 void poly_bounds(const float* c, double top, double& px, double& qx) {
     px = qx = 0;
     for (int k = 0; k <= 512; ++k) {
-        const double x = top * k / 512, x2 = x * x, q = c[1] * x2 + c[2] * x2 * x2;
-        px = fmax(px, fabs((c[0] + q) * x));
+        const double x = top * k / 512, x2 = x * x, q = c[0] + c[1] * x2 + c[2] * x2 * x2;
+        px = fmax(px, fabs(q * x));
         qx = fmax(qx, fabs(q));
     }
 }
 
-template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, int64_t grid, hipStream_t st) {
+template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStream_t st) {
     constexpr int smem = Cfg<T, SPLIT>::SMEM;
     static const hipError_t set = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (set != hipSuccess) return (int)set;
-    hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3((unsigned)grid), dim3(512), smem, st, ga);
+    const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
+    hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3(ga.ntiles < most ? ga.ntiles : most), dim3(512), smem, st, ga);
     return dino_launch_status();
 }
-template <int MODE> int launch_gemm(const GemmArgs& ga, int T, bool split, int64_t grid, hipStream_t st) {
-    if (T == 256) return split ? launch_as<MODE, 256, true>(ga, grid, st) : launch_as<MODE, 256, false>(ga, grid, st);
-    if (T == 192) return split ? launch_as<MODE, 192, true>(ga, grid, st) : launch_as<MODE, 192, false>(ga, grid, st);
-    return split ? launch_as<MODE, 128, true>(ga, grid, st) : launch_as<MODE, 128, false>(ga, grid, st);
+template <int MODE> int launch_gemm(GemmArgs& ga, int T, bool split, int64_t tiles, hipStream_t st) {
+    ga.ntiles = (int)tiles;
+    if (T == 256) return split ? launch_as<MODE, 256, true>(ga, st) : launch_as<MODE, 256, false>(ga, st);
+    return split ? launch_as<MODE, 128, true>(ga, st) : launch_as<MODE, 128, false>(ga, st);
 }
 
 }  // namespace
@@ -640,11 +797,13 @@ extern "C" int dino_ortho(const dino_ortho_item* items, int count, int steps, co
     char* w = (char*)workspace;
     Ws ws;
     ws.mats = (Mat*)(w + L.mats);
-    ws.map_sym = (int*)(w + L.maps[0]);
-    ws.map_rect = (int*)(w + L.maps[1]);
-    ws.map_prep = (int*)(w + L.maps[2]);
+    ws.sym = (Tile*)(w + L.sym);
+    ws.rect = (Tile*)(w + L.rect);
+    ws.map_prep = (int*)(w + L.map);
     ws.parts = (double*)(w + L.parts);
     ws.exps = (float*)(w + L.exps);
+    ws.tsym = L.tile[0];
+    ws.trect = L.tile[1];
     for (int k = 0; k < 2; ++k)
         for (int h = 0; h < 2; ++h) ws.x[k][h] = (f16*)(w + L.x + (2 * k + h) * L.xbytes);
     for (int h = 0; h < 2; ++h) {
@@ -671,16 +830,15 @@ extern "C" int dino_ortho(const dino_ortho_item* items, int count, int steps, co
     rc = dino_launch_status();
     for (int s = 0; s < steps && rc == DINO_OK; ++s) {
         const float* c = coeffs + 3 * s;
-        GemmArgs ga{ws, s & 1, split(s + 1), 0.f, (float)(sa[s] / ((double)SX * SX))};
+        GemmArgs ga{ws, s & 1, split(s + 1), 0, 0.f, (float)(sa[s] / ((double)SX * SX)), 0.f};
         rc = launch_gemm<GRAM>(ga, L.tile[0], split(s), L.ntile[0], st);
         if (rc != DINO_OK) break;
         ga.c0 = (float)(c[1] * sb[s] / sa[s]);
         ga.c1 = (float)(c[2] * sb[s] / (sa[s] * sa[s]));
+        ga.ca = (float)(c[0] * sb[s]);
         rc = launch_gemm<POLY>(ga, L.tile[0], split(s), L.ntile[0], st);
         if (rc != DINO_OK) break;
-        const double o = s + 1 == steps ? 1.0 / SX : 1.0;
-        ga.c0 = (float)(c[0] * o);
-        ga.c1 = (float)(o / sb[s]);
+        ga.c1 = (float)((s + 1 == steps ? 1.0 / SX : 1.0) / sb[s]);
         rc = s + 1 == steps ? launch_gemm<FINAL>(ga, L.tile[1], split(s), L.ntile[1], st)
                             : launch_gemm<UPDATE>(ga, L.tile[1], split(s), L.ntile[1], st);
     }
