@@ -39,7 +39,7 @@ struct Mat {
     void* out;
     int64_t in_batch, in_ld, out_batch, out_ld, xoff, aoff;
     int rows, cols, batch, dtype;
-    int tall, m, n, mp, np;                     // m <= n; mp, np: padded to 32 (zeros)
+    int tall, m, n, mp, np;                     // m <= n; mp, np: padded to 64 (zeros)
     int parts, part0, mat0;                     // partial sums of the norm: per matrix, first index; first matrix
     int preps;                                  // 64 x 64 tiles that a workgroup of the preparing kernel takes
     int sym0, rect0, prep0;                     // first tile of each kind
@@ -256,8 +256,14 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
     static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
-    static constexpr int OPB = T * BK * 2, STAGE = (SPLIT ? 4 : 2) * OPB;
-    static constexpr int S = SPLIT ? 2 : 4;                         // 128 KB (T = 256), 64 KB (T = 128)
+    // parts of a stage: hi and lo of one panel of 32, or (T = 128) two panels: fewer phases, which cost ~0.35 us each
+    static constexpr int KB = T == 128 && !SPLIT ? 2 : 1, NP = SPLIT ? 2 : KB;
+    static constexpr int OPB = T * BK * 2, STAGE = 2 * NP * OPB;
+#ifdef OT_DEEP
+    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : 4;
+#else
+    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : 2;        // 128 KB (T = 256), 64 KB (T = 128)
+#endif
     static constexpr int ND = T / 64;                               // DMAs a wave, stage and part (hi / lo)
     static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
     static constexpr int IMG = 16 * SUBM * 2;                       // image of 16 columns of it
@@ -298,7 +304,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Cfg<T, SPLIT> C;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, NP = SPLIT ? 2 : 1;
+    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, NP = C::NP, KB = C::KB;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -323,7 +329,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         const int r = (isP || SYM ? e * 16 : (e & 1) * 16) + (lane >> 2);
         vo[u] = r * 64 + (((lane & 3) ^ (isP || SYM ? fsw(r >> 2) : tkey(r))) << 4);
     }
-    u32x4 rsP[NP], rsQ[NP];
+    u32x4 rsP[SPLIT ? 2 : 1], rsQ[SPLIT ? 2 : 1];
     const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
     int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, islot = 0, issued = 0;
     Tile tn = load_tile(tiles + b0);                       // the tile after the one being requested
@@ -331,9 +337,9 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         imp = tn.mp;
         im0 = tn.m0;
         in0 = tn.n0;
-        itotal = (MODE == GRAM ? tn.np : tn.mp) / BK;
+        itotal = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
 #pragma unroll
-        for (int h = 0; h < NP; ++h) {
+        for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
             const f16* P = MODE == GRAM ? ws.x[ga.src][h] + tn.xo : MODE == POLY ? ws.a[h] + tn.ao : ws.b[h] + tn.ao;
             const f16* Q = MODE == POLY ? ws.a[h] + tn.ao : ws.x[ga.src][h] + tn.xo;
             rsP[h] = rsrc(P, tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
@@ -344,17 +350,20 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     open();
     auto issue = [&]() {
         if (ji < nmine) {
-            const int soP = (ik * imp + im0) * 64;
-            const int soQ = SYM ? (ik * imp + in0) * 64 : ((in0 >> 5) * imp + ik * 32) * 64;
 #pragma unroll
-            for (int h = 0; h < NP; ++h)
+            for (int h = 0; h < NP; ++h) {
+                const int kp = SPLIT ? ik : ik * KB + h;       // panel along the contraction
+                const int soP = (kp * imp + im0) * 64;
+                const int soQ = SYM ? (kp * imp + in0) * 64 : ((in0 >> 5) * imp + kp * 32) * 64;
 #pragma unroll
                 for (int u = 0; u < ND; ++u) {
                     const bool isP = u < ND / 2;
                     const int d = wave + 8 * u;
                     const int so = isP ? soP : SYM ? soQ : soQ + ((d - T / 16) >> 1) * imp * 64;
-                    dma16(lds0 + islot * C::STAGE + h * 2 * C::OPB + d * 1024, vo[u], isP ? rsP[h] : rsQ[h], so);
+                    dma16(lds0 + islot * C::STAGE + h * 2 * C::OPB + d * 1024, vo[u],
+                          isP ? rsP[SPLIT ? h : 0] : rsQ[SPLIT ? h : 0], so);
                 }
+            }
             ++issued;
             if (++ik == itotal) {
                 ik = 0;
@@ -365,9 +374,9 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     };
     auto landed = [&](int s) {       // my DMAs of stage s are done
         const int younger = issued - 1 - s;
-        if (S == 4 && younger >= 3) wait_vmcnt<NP * ND * 3>();
-        else if (S == 4 && younger == 2) wait_vmcnt<NP * ND * 2>();
-        else if (younger >= 1) wait_vmcnt<NP * ND>();
+        // (at most S - 1 stages are younger; where the stream ends the count falls below S - 2: then all but one)
+        if (younger >= S - 2) wait_vmcnt<NP * ND * (S - 2)>();
+        else if (S == 4 && younger == 1) wait_vmcnt<NP * ND>();
         else wait_vmcnt<0>();
     };
 
@@ -421,7 +430,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         if (SPLIT) {
             mm(NP - 1, 0);
             mm(0, NP - 1);
-        }
+        } else if (NP > 1) mm(NP - 1, NP - 1);
         mm(0, 0);
     };
     auto phase = [&]() {
@@ -441,7 +450,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         const float c0 = ga.c0 * e2, c1 = MODE == POLY ? ga.c1 * e2 * e2 : MODE == FINAL ? ga.c1 * e1 : ga.c1;
         const int wm0 = d.m0 + wm * C::SUBM, wn0 = d.n0 + wn * C::SUBN;
         const int nend = SYM ? mp : np;
-        // where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 32, so a
+        // where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 64, so a
         // fragment is inside as a whole or outside as a whole)
         const int vlane = i * 64 + g * 8;
         auto upart = [&](int ni) {           // (+ 1024 mi)
@@ -451,15 +460,16 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         if (MODE == POLY) {
             // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads a neighbour or
             // zero and is not stored)
-            __amdgpu_buffer_rsrc_t rs[NP];
+            constexpr int EP = SPLIT ? 2 : 1;
+            __amdgpu_buffer_rsrc_t rs[EP];
 #pragma unroll
-            for (int h = 0; h < NP; ++h) rs[h] = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a[h] + d.ao), 0, mp * mp * 2, 0x00020000);
+            for (int h = 0; h < EP; ++h) rs[h] = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a[h] + d.ao), 0, mp * mp * 2, 0x00020000);
             constexpr int PART = MI / (SPLIT ? 4 : 2);
 #pragma unroll
             for (int q = 0; q < MI; q += PART) {
-                f16x4 el[NP][PART][NI];
+                f16x4 el[EP][PART][NI];
 #pragma unroll
-                for (int h = 0; h < NP; ++h)
+                for (int h = 0; h < EP; ++h)
 #pragma unroll
                     for (int mi = 0; mi < PART; ++mi)
 #pragma unroll
@@ -472,18 +482,19 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float x = (float)el[0][mi][ni][r];
-                            if (SPLIT) x += (float)el[NP - 1][mi][ni][r];
+                            if (SPLIT) x += (float)el[EP - 1][mi][ni][r];
                             acc[q + mi][ni][r] = fmaf(c0, x, acc[q + mi][ni][r] * c1);
                         }
             }
             if (d.m0 == d.n0) {
+                int off = wm0 + i - wn0 - 4 * g;
+                asm volatile("" : "+v"(off));        // (or the 128 comparisons, the same for every tile, are kept in registers)
 #pragma unroll
                 for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
                     for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (wm0 + mi * 16 + i == wn0 + 16 * ni + 4 * g + r) acc[mi][ni][r] += ga.ca;
+                        for (int r = 0; r < 4; ++r) acc[mi][ni][r] += off == 16 * (ni - mi) + r ? ga.ca : 0.f;
             }
         } else {
 #pragma unroll
@@ -599,7 +610,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     // tile that ended with s is finished by both in phase 2s + 2, where stage s + S is requested into the slot of s.
     for (int s = 0; s < S - 1; ++s) issue();
     Tile cur = load_tile(tiles + b0), nxt = load_tile(tiles + b0 + (nmine > 1 ? G : 0));
-    int total = (MODE == GRAM ? cur.np : cur.mp) / BK, j = 0, k = 0;
+    int total = (MODE == GRAM ? cur.np : cur.mp) / (BK * KB), j = 0, k = 0;
     float e1 = load_const(ws.exps + cur.all);
     landed(0);
     phase();
@@ -622,7 +633,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
             cur = nxt;
             e1 = load_const(ws.exps + cur.all);
             if (j + 1 < nmine) nxt = load_tile(tiles + b0 + (j + 1) * G);
-            total = (MODE == GRAM ? cur.np : cur.mp) / BK;
+            total = (MODE == GRAM ? cur.np : cur.mp) / (BK * KB);
             k = 0;
         }
         if (late) phase();
@@ -652,8 +663,8 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         q.tall = s.rows > s.cols;
         q.m = q.tall ? s.cols : s.rows;
         q.n = q.tall ? s.rows : s.cols;
-        q.mp = (int)up(q.m, 32);
-        q.np = (int)up(q.n, 32);
+        q.mp = (int)up(q.m, 64);
+        q.np = (int)up(q.n, 64);
         if ((int64_t)q.mp * q.np * 2 >= (1ll << 31)) return DINO_ERR_TOO_LARGE;
         int64_t p = ((int64_t)q.m * q.n + 16383) / 16384;
         if (p > 256) p = 256;
@@ -678,8 +689,8 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         for (int T = 256; T >= 128; T /= 2) {
             double work = 0, tiles = 0;
             for (int i = 0; i < count; ++i) {
-                const int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 32);
-                const int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 32);
+                const int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 64);
+                const int64_t n = up(items[i].rows < items[i].cols ? items[i].cols : items[i].rows, 64);
                 const double tm = (double)((m + T - 1) / T), tn = (double)((n + T - 1) / T);
                 const double k = kind ? tm * tn * items[i].batch : tm * (tm + 1) / 2 * items[i].batch;
                 tiles += k;
@@ -702,7 +713,7 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         std::stable_sort(order, order + count, [&](int a, int b) { return kind ? lo_side(a) > lo_side(b) : hi_side(a) > hi_side(b); });
         for (int o = 0; o < count; ++o) {
             const int i = order[o], T = L.tile[kind];
-            const int64_t m = up(lo_side(i), 32), n = up(hi_side(i), 32), tm = (m + T - 1) / T;
+            const int64_t m = up(lo_side(i), 64), n = up(hi_side(i), 64), tm = (m + T - 1) / T;
             int64_t& at = kind ? rect : sym;
             if (out) (kind ? out[i].rect0 : out[i].sym0) = (int)at;
             at += items[i].batch * (kind ? tm * ((n + T - 1) / T) : tm * (tm + 1) / 2);
@@ -741,7 +752,12 @@ template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStre
     static const hipError_t set = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (set != hipSuccess) return (int)set;
-    const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
+    #ifdef OT_DEEP
+    const int most = 256;
+#else
+    const int most = 256 * (T == 128 ? 2 : 1);
+#endif
+          // what the CUs hold at once
     hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3(ga.ntiles < most ? ga.ntiles : most), dim3(512), smem, st, ga);
     return dino_launch_status();
 }
