@@ -7,11 +7,13 @@
 // Number formats.  The operands of the matrix instructions are fp16: every |x| is at most the largest singular value
 // (about 1.2), so the range that bf16 pays three bits for is not needed; X, A, B are kept times powers of two that put
 // them in the middle of fp16's range (X's by the matrix: an update that is small against eps starts at |U| / eps and
-// ends at most `gain` = prod max(1, a) times that, so it is held 2^e times larger).  All sums are fp32 (the norm's fp64).  A rounding error made in step i grows by
-// a^(steps - 1 - i) in the directions of small singular values (3.44^4 = 140 from the first of five steps), against an
-// answer that is O(1) there.  While that factor is above SPLIT_ABOVE the operands are hi + lo pairs of fp16 (22 bits;
-// products hi hi + hi lo + lo hi, three passes of the same loop); after that plain fp16.  On an update of four strong
-// directions over noise the result is then 0.003 off 64 bits, with plain fp16 throughout 0.04, with bf16 0.33.
+// ends at most `gain` = prod max(1, a) times that, so it is held 2^e times larger).  All sums are fp32 (the norm's fp64).
+// A rounding of X in step i is noise in every direction, and grows by a^(steps - 1 - i) in those of small singular
+// values (3.44^4 = 140 from the first of five steps), against an answer that is O(1) there.  While that factor is above
+// SPLIT_ABOVE, X is a hi + lo pair of fp16 (22 bits) in X <- B X: two products.  A and B need no more than fp16: their
+// roundings, multiplied by X, stay in the directions that X has.  On an update of four strong directions over 0.01 of
+// noise the result is 0.0018 off 64 bits with pairs in three of five steps (0.0053 in two, 0.0010 in four), 0.042
+// without, 0.33 with bf16 throughout; its own rounding to bf16 is 0.0017.
 #include <math.h>
 #include <stdlib.h>
 
@@ -31,7 +33,7 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 constexpr int BK = 32, NTHR = 256;
 constexpr int ITEMS = 16;                       // items described by one launch of the norm kernel
 constexpr float SX = 4096.f;                    // X is stored times this
-constexpr double SPLIT_ABOVE = 16.0;
+constexpr double SPLIT_ABOVE = 8.0;
 
 // One item: `batch` matrices of one shape.  Offsets in elements of the region of their kind.
 struct Mat {
@@ -72,7 +74,7 @@ struct Ws {                                     // regions of the workspace
     double* parts;
     float* exps;                                // 2^-e of each matrix
     int tsym, trect;                            // tile sizes
-    f16 *x[2][2], *a[2], *b[2];                 // [buffer][hi / lo]
+    f16 *x[2][2], *a, *b;                       // X: [buffer][hi / lo]
 };
 
 DEVI double block_sum_f64(double v, double* red) {
@@ -247,27 +249,24 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 //   FINAL   the last UPDATE: into the caller's matrix as bf16
 // (a on B's diagonal instead of a X in the update: no second read of X.)
 // Operands go global -> LDS by DMA in a ring of S stages of 32 along the contraction, one stream of stages over all tiles of
-// the workgroup: the next tile's first stages are on their way while this one's results leave.  With SPLIT a stage
-// holds the hi and lo parts of both operands and feeds three products (hi hi, hi lo, lo hi): 3 products for 2 loads.  The
-// path from L2 to the CUs bounds these products (about 9.4 TB/s: T / 2 operations a byte), hence the large tiles.
+// the workgroup: the next tile's first stages are on their way while this one's results leave.  With SPLIT (an UPDATE) a
+// stage holds the hi and the lo part of X and feeds two products.  The path from L2 to the CUs bounds these products (about
+// 9.4 TB/s: T / 2 operations a byte), hence the large tiles.
 // The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
 // multiplies.  Waves 4..7 ("late") run one phase behind waves 0..3: stage s is read in phases 2s and 2s + 1, its slot is
 // refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
     static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
-    // parts of a stage: hi and lo of one panel of 32, or (T = 128) two panels: fewer phases, which cost ~0.35 us each
-    static constexpr int KB = T == 128 && !SPLIT ? 2 : 1, NP = SPLIT ? 2 : KB;
-    static constexpr int OPB = T * BK * 2, STAGE = 2 * NP * OPB;
-#ifdef OT_DEEP
-    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : 4;
-#else
-    static constexpr int S = T == 256 ? (SPLIT ? 2 : 4) : 2;        // 128 KB (T = 256), 64 KB (T = 128)
-#endif
-    static constexpr int ND = T / 64;                               // DMAs a wave, stage and part (hi / lo)
+    // parts of a stage: one panel of P and one of Q (SPLIT: its hi and lo), or (T = 128) two panels of both: fewer
+    // phases, which cost about 0.35 us each
+    static constexpr int KB = T == 128 && !SPLIT ? 2 : 1, PP = KB, QP = SPLIT ? 2 : KB;
+    static constexpr int OPB = T * BK * 2, STAGE = (PP + QP) * OPB;
+    static constexpr int S = SPLIT ? 3 : T == 256 ? 4 : 2;          // 128 to 144 KB (T = 256), 64 to 72 KB (T = 128)
+    static constexpr int ND = T / 128;                              // DMAs a wave and part
     static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
-    static constexpr int IMG = 16 * SUBM * 2;                       // image of 16 columns of it
-    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 160 KB / 80 KB: one / two workgroups a CU
+    static constexpr int IMG = SPLIT ? 0 : 16 * SUBM * 2;           // image of 16 columns of it (UPDATE has none)
+    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 144 to 160 KB / 72 to 80 KB: one / two workgroups a CU
 };
 // The DMA is written in assembly: behind the builtin the compiler waits for ALL requests before every transposing LDS
 // read, which may alias what is being filled for all it knows.  It has no register result; the waits are landed()'s.
@@ -304,7 +303,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Cfg<T, SPLIT> C;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, NP = C::NP, KB = C::KB;
+    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, KB = C::KB, PP = C::PP, QP = C::QP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -321,15 +320,14 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     // DMA of a wave moves 1 KB in one piece.  Chunks are permuted by a key of the row so that no read meets itself
     // in a bank.  Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not
     // stored, see them.  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
-    int vo[ND];
+    int voP[ND], voQ[ND];
 #pragma unroll
     for (int u = 0; u < ND; ++u) {
-        const bool isP = u < ND / 2;
-        const int e = wave + 8 * u - (isP ? 0 : T / 16);
-        const int r = (isP || SYM ? e * 16 : (e & 1) * 16) + (lane >> 2);
-        vo[u] = r * 64 + (((lane & 3) ^ (isP || SYM ? fsw(r >> 2) : tkey(r))) << 4);
+        const int e = wave + 8 * u, r = e * 16 + (lane >> 2), t = (e & 1) * 16 + (lane >> 2);
+        voP[u] = r * 64 + (((lane & 3) ^ fsw(r >> 2)) << 4);
+        voQ[u] = SYM ? voP[u] : t * 64 + (((lane & 3) ^ tkey(t)) << 4);
     }
-    u32x4 rsP[SPLIT ? 2 : 1], rsQ[SPLIT ? 2 : 1];
+    u32x4 rsP, rsQ[SPLIT ? 2 : 1];
     const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
     int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, islot = 0, issued = 0;
     Tile tn = load_tile(tiles + b0);                       // the tile after the one being requested
@@ -338,32 +336,30 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         im0 = tn.m0;
         in0 = tn.n0;
         itotal = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
+        rsP = rsrc(MODE == GRAM ? ws.x[ga.src][0] + tn.xo : MODE == POLY ? ws.a + tn.ao : ws.b + tn.ao,
+                   tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
 #pragma unroll
-        for (int h = 0; h < (SPLIT ? 2 : 1); ++h) {
-            const f16* P = MODE == GRAM ? ws.x[ga.src][h] + tn.xo : MODE == POLY ? ws.a[h] + tn.ao : ws.b[h] + tn.ao;
-            const f16* Q = MODE == POLY ? ws.a[h] + tn.ao : ws.x[ga.src][h] + tn.xo;
-            rsP[h] = rsrc(P, tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
-            rsQ[h] = rsrc(Q, tn.mp * (MODE == POLY ? tn.mp : tn.np) * 2);
-        }
+        for (int h = 0; h < (SPLIT ? 2 : 1); ++h)
+            rsQ[h] = rsrc(MODE == POLY ? ws.a + tn.ao : ws.x[ga.src][h] + tn.xo, tn.mp * (MODE == POLY ? tn.mp : tn.np) * 2);
         if (ji + 1 < nmine) tn = load_tile(tiles + b0 + (ji + 1) * G);
     };
     open();
     auto issue = [&]() {
         if (ji < nmine) {
+            const unsigned at = lds0 + islot * C::STAGE + wave * 1024;
 #pragma unroll
-            for (int h = 0; h < NP; ++h) {
-                const int kp = SPLIT ? ik : ik * KB + h;       // panel along the contraction
-                const int soP = (kp * imp + im0) * 64;
-                const int soQ = SYM ? (kp * imp + in0) * 64 : ((in0 >> 5) * imp + kp * 32) * 64;
+            for (int h = 0; h < PP; ++h)
+#pragma unroll
+                for (int u = 0; u < ND; ++u)
+                    dma16(at + h * C::OPB + u * 8192, voP[u], rsP, ((ik * KB + h) * imp + im0) * 64);
+#pragma unroll
+            for (int h = 0; h < QP; ++h)
 #pragma unroll
                 for (int u = 0; u < ND; ++u) {
-                    const bool isP = u < ND / 2;
-                    const int d = wave + 8 * u;
-                    const int so = isP ? soP : SYM ? soQ : soQ + ((d - T / 16) >> 1) * imp * 64;
-                    dma16(lds0 + islot * C::STAGE + h * 2 * C::OPB + d * 1024, vo[u],
-                          isP ? rsP[SPLIT ? h : 0] : rsQ[SPLIT ? h : 0], so);
+                    const int kp = SPLIT ? ik : ik * KB + h;   // panel along the contraction
+                    const int so = SYM ? (kp * imp + in0) * 64 : (((in0 >> 5) + ((wave + 8 * u) >> 1)) * imp + kp * 32) * 64;
+                    dma16(at + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h : 0], so);
                 }
-            }
             ++issued;
             if (++ik == itotal) {
                 ik = 0;
@@ -375,8 +371,8 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     auto landed = [&](int s) {       // my DMAs of stage s are done
         const int younger = issued - 1 - s;
         // (at most S - 1 stages are younger; where the stream ends the count falls below S - 2: then all but one)
-        if (younger >= S - 2) wait_vmcnt<NP * ND * (S - 2)>();
-        else if (S == 4 && younger == 1) wait_vmcnt<NP * ND>();
+        if (younger >= S - 2) wait_vmcnt<(PP + QP) * ND * (S - 2)>();
+        else if (S == 4 && younger == 1) wait_vmcnt<(PP + QP) * ND>();
         else wait_vmcnt<0>();
     };
 
@@ -389,23 +385,23 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     };
     clear();
     const int rp = wm * C::SUBM + i, offP = rp * 64 + ((g ^ fsw(rp >> 2)) << 4);
-    const int rq = wn * C::SUBN + i, offQ = C::OPB + rq * 64 + ((g ^ fsw(rq >> 2)) << 4);
+    const int rq = wn * C::SUBN + i, offQ = PP * C::OPB + rq * 64 + ((g ^ fsw(rq >> 2)) << 4);
     int offT[NI];
 #pragma unroll
     for (int ni = 0; ni < NI; ++ni) {
         const int row = 8 * g + (i >> 2), col = wn * C::SUBN + ni * 16, ch = (col & 31) / 8 + ((i & 3) >> 1);
-        offT[ni] = C::OPB + (col >> 5) * 2048 + row * 64 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
+        offT[ni] = PP * C::OPB + (col >> 5) * 2048 + row * 64 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
     }
-    u32x4 fp[NP][MI], fq[NP][NI];
+    u32x4 fp[PP][MI], fq[QP][NI];
     int slot = 0;
     auto read = [&]() {
         const char* st = smem + slot * C::STAGE;
         slot = slot + 1 == S ? 0 : slot + 1;
 #pragma unroll
-        for (int h = 0; h < NP; ++h) {
-            const char* sh = st + h * 2 * C::OPB;
+        for (int h = 0; h < QP; ++h)
 #pragma unroll
             for (int x = 0; x < NI; ++x) {
+                const char* sh = st + h * C::OPB;
                 if (SYM) fq[h][x] = *(const u32x4*)(sh + offQ + x * 1024);
                 else {
                     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sh + offT[x])));
@@ -414,24 +410,20 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                 }
             }
 #pragma unroll
-            for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(sh + offP + x * 1024);
-        }
+        for (int h = 0; h < PP; ++h)
+#pragma unroll
+            for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(st + h * C::OPB + offP + x * 1024);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     auto multiply = [&]() {
-        auto mm = [&](int hp, int hq) {
+#pragma unroll
+        for (int h = QP - 1; h >= 0; --h)
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
                     acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        __builtin_bit_cast(f16x8, fq[hq][ni]), __builtin_bit_cast(f16x8, fp[hp][mi]), acc[mi][ni], 0, 0, 0);
-        };
-        if (SPLIT) {
-            mm(NP - 1, 0);
-            mm(0, NP - 1);
-        } else if (NP > 1) mm(NP - 1, NP - 1);
-        mm(0, 0);
+                        __builtin_bit_cast(f16x8, fq[h][ni]), __builtin_bit_cast(f16x8, fp[SPLIT ? 0 : h][mi]), acc[mi][ni], 0, 0, 0);
     };
     auto phase = [&]() {
         asm volatile("" ::: "memory");
@@ -460,31 +452,23 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         if (MODE == POLY) {
             // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads a neighbour or
             // zero and is not stored)
-            constexpr int EP = SPLIT ? 2 : 1;
-            __amdgpu_buffer_rsrc_t rs[EP];
-#pragma unroll
-            for (int h = 0; h < EP; ++h) rs[h] = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a[h] + d.ao), 0, mp * mp * 2, 0x00020000);
-            constexpr int PART = MI / (SPLIT ? 4 : 2);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a + d.ao), 0, mp * mp * 2, 0x00020000);
+            constexpr int PART = MI / 2;
 #pragma unroll
             for (int q = 0; q < MI; q += PART) {
-                f16x4 el[EP][PART][NI];
+                f16x4 el[PART][NI];
 #pragma unroll
-                for (int h = 0; h < EP; ++h)
+                for (int mi = 0; mi < PART; ++mi)
 #pragma unroll
-                    for (int mi = 0; mi < PART; ++mi)
-#pragma unroll
-                        for (int ni = 0; ni < NI; ++ni)
-                            el[h][mi][ni] = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rs[h], vlane + (q + mi) * 1024, upart(ni), 0));
+                    for (int ni = 0; ni < NI; ++ni)
+                        el[mi][ni] = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rs, vlane + (q + mi) * 1024, upart(ni), 0));
 #pragma unroll
                 for (int mi = 0; mi < PART; ++mi)
 #pragma unroll
                     for (int ni = 0; ni < NI; ++ni)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float x = (float)el[0][mi][ni][r];
-                            if (SPLIT) x += (float)el[EP - 1][mi][ni][r];
-                            acc[q + mi][ni][r] = fmaf(c0, x, acc[q + mi][ni][r] * c1);
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            acc[q + mi][ni][r] = fmaf(c0, (float)el[mi][ni][r], acc[q + mi][ni][r] * c1);
             }
             if (d.m0 == d.n0) {
                 int off = wm0 + i - wn0 - 4 * g;
@@ -564,17 +548,12 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                     for (int r = 0; r < 4; ++r) acc[mi][ni][r] -= (float)(f16)acc[mi][ni][r];
         };
         if (SYM) {
-            f16* const* o = MODE == GRAM ? ws.a : ws.b;
-            put(o[0] + d.ao);
-            if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)(o[0] + d.ao), mp, mp, mp, true);
-            if (SPLIT) {
-                take_hi();
-                put(o[1] + d.ao);
-                if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)(o[1] + d.ao), mp, mp, mp, true);
-            }
+            f16* o = (MODE == GRAM ? ws.a : ws.b) + d.ao;
+            put(o);
+            if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)o, mp, mp, mp, true);
         } else if (MODE == UPDATE) {
             put(ws.x[ga.src ^ 1][0] + d.xo);
-            if (SPLIT && ga.split_next) {
+            if (SPLIT && ga.split_next) {          // (pairs are used from the first step on)
                 take_hi();
                 put(ws.x[ga.src ^ 1][1] + d.xo);
             }
@@ -732,7 +711,7 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
     L.xbytes = up(2 * xo, 256);
     L.abytes = up(2 * ao, 256);
     L.x = take(4 * L.xbytes);
-    L.a = take(4 * L.abytes);
+    L.a = take(2 * L.abytes);
     L.bytes = at;
     return DINO_OK;
 }
@@ -752,19 +731,14 @@ template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStre
     static const hipError_t set = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (set != hipSuccess) return (int)set;
-    #ifdef OT_DEEP
-    const int most = 256;
-#else
-    const int most = 256 * (T == 128 ? 2 : 1);
-#endif
-          // what the CUs hold at once
+        const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
     hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3(ga.ntiles < most ? ga.ntiles : most), dim3(512), smem, st, ga);
     return dino_launch_status();
 }
 template <int MODE> int launch_gemm(GemmArgs& ga, int T, bool split, int64_t tiles, hipStream_t st) {
     ga.ntiles = (int)tiles;
-    if (T == 256) return split ? launch_as<MODE, 256, true>(ga, st) : launch_as<MODE, 256, false>(ga, st);
-    return split ? launch_as<MODE, 128, true>(ga, st) : launch_as<MODE, 128, false>(ga, st);
+    if (MODE == UPDATE && split) return T == 256 ? launch_as<UPDATE, 256, true>(ga, st) : launch_as<UPDATE, 128, true>(ga, st);
+    return T == 256 ? launch_as<MODE, 256, false>(ga, st) : launch_as<MODE, 128, false>(ga, st);
 }
 
 }  // namespace
@@ -822,10 +796,8 @@ extern "C" int dino_ortho(const dino_ortho_item* items, int count, int steps, co
     ws.trect = L.tile[1];
     for (int k = 0; k < 2; ++k)
         for (int h = 0; h < 2; ++h) ws.x[k][h] = (f16*)(w + L.x + (2 * k + h) * L.xbytes);
-    for (int h = 0; h < 2; ++h) {
-        ws.a[h] = (f16*)(w + L.a + h * L.abytes);
-        ws.b[h] = (f16*)(w + L.a + (2 + h) * L.abytes);
-    }
+    ws.a = (f16*)(w + L.a);
+    ws.b = (f16*)(w + L.a + L.abytes);
     const hipStream_t st = (hipStream_t)stream;
     for (int i0 = 0; i0 < count; i0 += ITEMS) {
         Setup su;
@@ -847,15 +819,15 @@ extern "C" int dino_ortho(const dino_ortho_item* items, int count, int steps, co
     for (int s = 0; s < steps && rc == DINO_OK; ++s) {
         const float* c = coeffs + 3 * s;
         GemmArgs ga{ws, s & 1, split(s + 1), 0, 0.f, (float)(sa[s] / ((double)SX * SX)), 0.f};
-        rc = launch_gemm<GRAM>(ga, L.tile[0], split(s), L.ntile[0], st);
+        rc = launch_gemm<GRAM>(ga, L.tile[0], false, L.ntile[0], st);
         if (rc != DINO_OK) break;
         ga.c0 = (float)(c[1] * sb[s] / sa[s]);
         ga.c1 = (float)(c[2] * sb[s] / (sa[s] * sa[s]));
         ga.ca = (float)(c[0] * sb[s]);
-        rc = launch_gemm<POLY>(ga, L.tile[0], split(s), L.ntile[0], st);
+        rc = launch_gemm<POLY>(ga, L.tile[0], false, L.ntile[0], st);
         if (rc != DINO_OK) break;
         ga.c1 = (float)((s + 1 == steps ? 1.0 / SX : 1.0) / sb[s]);
-        rc = s + 1 == steps ? launch_gemm<FINAL>(ga, L.tile[1], split(s), L.ntile[1], st)
+        rc = s + 1 == steps ? launch_gemm<FINAL>(ga, L.tile[1], false, L.ntile[1], st)   // (the last step's errors do not grow)
                             : launch_gemm<UPDATE>(ga, L.tile[1], split(s), L.ntile[1], st);
     }
     return rc;
