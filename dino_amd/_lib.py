@@ -83,6 +83,8 @@ SIGNATURES = {
     "dino_adamw_ema": [P, P, P, P, P, P, P, P, I, P, P, F, F, F, F, F, P],
     "dino_ortho_workspace": [ctypes.POINTER(OrthoItem), I, ctypes.POINTER(c_int64)],
     "dino_ortho": [ctypes.POINTER(OrthoItem), I, I, ctypes.POINTER(c_float), ctypes.c_double, P, L, P],
+    "dino_muon_momentum": [P, P, P, P, I, P, P, F, I, P],
+    "dino_muon_apply": [P, P, P, I, P, P],
     "dino_ema": [P, P, P, L, F, F, P],
     "dino_cast_bf16": [P, P, L, P],
     "dino_transpose_batched": [I, P, P, P, I, P],

@@ -129,6 +129,38 @@ class DINOLoss(nn.Module):
         ops.center_update(self._buffers["center"].view(-1), self._acc, self.center_momentum,
                           1.0 / (nrows * world))
 
+    @torch.no_grad()
+    def watch(self, student_output, teacher_output, it):
+        """What the loss value does not show, from one pass over each output (ops.logprob_fwd), as 0-dim tensors on the
+        device (nothing is synchronised):
+          teacher_entropy   mean entropy of the centred, sharpened teacher rows -- 0: one prototype for each crop,
+                            log(out_dim): none at all; collapse shows here first
+          student_entropy   the same of the student rows at its temperature
+          agreement         share of student rows whose best prototype is that of a teacher view of their image
+          assigned_log_prob mean log probability that the student gives to the other views' best prototypes
+          prototypes_used   number of different best prototypes over the teacher rows
+        The centre is the module's present one.  Call it beside forward(); it changes nothing."""
+        if getattr(student_output, "_dino_lazy", None) is not None:
+            raise ValueError("DINOLoss.watch needs the student's logits (fused_head_loss gives its bottleneck instead)")
+        if student_output.shape[0] != self.ncrops * (teacher_output.shape[0] // 2):
+            raise ValueError(f"student rows {student_output.shape[0]} != ncrops*B = "
+                             f"{self.ncrops}*{teacher_output.shape[0] // 2}")
+        temp, t_dim = float(self.teacher_temp_schedule[it]), teacher_output.shape[1]
+        center = self.center.detach().to(torch.float32).reshape(-1).contiguous()
+        t = ops.logprob_fwd(teacher_output.detach(), None, center=center, temp=temp, topk=1)
+        B = teacher_output.shape[0] // 2
+        best = t.top_index.view(2, B)
+        targets = best.t().repeat(self.ncrops, 1)        # both views' best prototypes, for every crop of the image
+        targets[:B, 0] = -1                              # a global crop is not held to its own view
+        targets[B:2 * B, 1] = -1
+        s = ops.logprob_fwd(student_output.detach(), targets.contiguous(), temp=self.student_temp, topk=1)
+        given = targets >= 0
+        used = torch.zeros(t_dim, dtype=torch.float32, device=best.device).index_fill_(0, best.reshape(-1), 1.0)
+        return {"teacher_entropy": t.entropy.mean(), "student_entropy": s.entropy.mean(),
+                "agreement": ((s.top_index == targets) & given).any(1).float().mean(),
+                "assigned_log_prob": s.log_prob.sum() / given.sum(),
+                "prototypes_used": used.sum()}
+
     def pop_wait_ms(self):
         """Sum of the event-timed centre-join waits since the last call (set .timing = True first)."""
         ev = self.__dict__.get("_wait_events") or []

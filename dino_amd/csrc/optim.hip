@@ -129,6 +129,46 @@ __global__ __launch_bounds__(256) void adamw_ema_kernel(
     }
 }
 
+// Muon's two streaming passes, over the chunks of its matrices; a tensor takes part when hp[5] != 0 (it has a gradient).
+// buf = mu buf + g;  u = nesterov ? g + mu buf : buf  (20 bytes an element, the rate of memory)
+__global__ __launch_bounds__(256) void muon_momentum_kernel(const float* __restrict__ grad, float* __restrict__ buf,
+                                                            float* __restrict__ update, const Chunk* __restrict__ chunks,
+                                                            const float* __restrict__ hp, const float* __restrict__ coef,
+                                                            float mu, int nesterov) {
+    const Chunk c = chunks[blockIdx.x];
+    if (hp[c.tensor * 8 + 5] == 0.f) return;
+    const float gk = coef ? coef[c.tensor] : 1.f;
+    for (int64_t i = c.start + threadIdx.x * 8; i < c.start + c.len; i += 256 * 8) {
+        float g[8], b[8], u[8];
+        load8<float>(grad + i, g);
+        load8<float>(buf + i, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float ge = g[e] * gk;
+            b[e] = fmaf(mu, b[e], ge);
+            u[e] = nesterov ? fmaf(mu, b[e], ge) : b[e];
+        }
+        store8<float>(buf + i, b);
+        store8<float>(update + i, u);
+    }
+}
+// p = p (1 - lr wd) - lr scale o,  o: the orthogonalised update (bf16)
+__global__ __launch_bounds__(256) void muon_apply_kernel(float* __restrict__ param, const bf16* __restrict__ ortho,
+                                                         const Chunk* __restrict__ chunks, const float* __restrict__ hp) {
+    const Chunk c = chunks[blockIdx.x];
+    const float* h = hp + c.tensor * 8;
+    if (h[5] == 0.f) return;
+    const float decay = 1.f - h[0] * h[1], step = h[0] * h[6];
+    for (int64_t i = c.start + threadIdx.x * 8; i < c.start + c.len; i += 256 * 8) {
+        float p[8], o[8];
+        load8<float>(param + i, p);
+        load8<bf16>(ortho + i, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = fmaf(-step, o[e], p[e] * decay);
+        store8<float>(param + i, p);
+    }
+}
+
 __global__ __launch_bounds__(256) void ema_kernel(float* __restrict__ teacher,
                                                   const float* __restrict__ student,
                                                   bf16* __restrict__ tshadow, int64_t n8, float m,
@@ -298,5 +338,23 @@ extern "C" int dino_transpose_batched(int dtype, const float* src_base, void* ds
                            (float*)dst_base, (const Mat*)table, nmat);
     else
         return DINO_ERR_BADARG;
+    return dino_launch_status();
+}
+
+extern "C" int dino_muon_momentum(const float* grad, float* momentum, float* update, const int64_t* chunks, int nchunks,
+                                  const float* hp, const float* coef, float mu, int nesterov, void* stream) {
+    DINO_CHECK_ARG(grad && momentum && update && chunks && hp && nchunks >= 0);
+    if (nchunks == 0) return DINO_OK;
+    hipLaunchKernelGGL(muon_momentum_kernel, dim3(nchunks), dim3(256), 0, (hipStream_t)stream, grad, momentum, update,
+                       (const Chunk*)chunks, hp, coef, mu, nesterov);
+    return dino_launch_status();
+}
+
+extern "C" int dino_muon_apply(float* param, const void* ortho, const int64_t* chunks, int nchunks, const float* hp,
+                               void* stream) {
+    DINO_CHECK_ARG(param && ortho && chunks && hp && nchunks >= 0);
+    if (nchunks == 0) return DINO_OK;
+    hipLaunchKernelGGL(muon_apply_kernel, dim3(nchunks), dim3(256), 0, (hipStream_t)stream, param, (const bf16*)ortho,
+                       (const Chunk*)chunks, hp);
     return dino_launch_status();
 }

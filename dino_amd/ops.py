@@ -579,51 +579,92 @@ NS_COEFFS = (3.4445, -4.7750, 2.0315)     # quintic that takes singular values o
 ORTHO_MAX_STEPS = 16
 
 
+class OrthoPlan:
+    """The checked operands of orthogonalize() for buffers that stay where they are (an optimiser's): run() only launches.
+    Holds the tensors; keeps no workspace."""
+
+    def __init__(self, updates, out=None, *, steps=5, coeffs=NS_COEFFS, eps=1e-7):
+        ups = list(updates)
+        _req(isinstance(steps, int) and 1 <= steps <= ORTHO_MAX_STEPS, f"steps: 1 to {ORTHO_MAX_STEPS}", steps)
+        coeffs = list(coeffs)
+        rows = [list(c) for c in coeffs] if coeffs and not isinstance(coeffs[0], (int, float)) else [coeffs] * steps
+        _req(len(rows) == steps and all(len(c) == 3 for c in rows), "coeffs: (a, b, c), or one triple per step", coeffs)
+        _req(isinstance(eps, (int, float)) and 0.0 <= eps < 1e30, "eps", eps)
+        outs = [None] * len(ups) if out is None else list(out)
+        _req(len(outs) == len(ups), "out: one for each update")
+        self.out, self._updates, self._steps, self._eps = [], ups, steps, float(eps)
+        if not ups:
+            return
+        _dev(*ups, *outs)
+        self._dev = dev = ups[0].device
+        self._items = (_lib.OrthoItem * len(ups))()
+        with _on(dev):
+            for q, u, o in zip(self._items, ups, outs):
+                shape = u.shape
+                _req(len(shape) in (2, 3) and u.device == dev, "updates: [rows, cols] or [batch, rows, cols] on one device",
+                     shape)
+                if o is None:
+                    o = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+                _req(o.shape == shape and o.dtype is torch.bfloat16 and o.device == dev, "out: bf16 of the update's shape")
+                r, c = shape[-2], shape[-1]
+                _req(r > 0 and c > 0, "an empty matrix", shape)
+                q.inp, q.in_batch, q.in_ld = self._place(u, r, c)
+                q.out, q.out_batch, q.out_ld = self._place(o, r, c)
+                q.rows, q.cols, q.batch, q.dtype = r, c, shape[0] if len(shape) == 3 else 1, dt_code(u.dtype)
+                self.out.append(o)
+            self._coeffs = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
+            need = ctypes.c_int64(0)
+            check(_lib.load().dino_ortho_workspace(self._items, len(ups), ctypes.byref(need)), "dino_ortho_workspace")
+            self._need = need.value
+
+    @staticmethod
+    def _place(t, r, c):
+        """(address, stride between matrices, between rows)"""
+        st = t.stride()
+        _req((st[-1] == 1 or c == 1) and (st[-2] >= c or r == 1), "columns side by side, rows apart", t.shape, st)
+        _req(len(st) == 2 or t.shape[0] <= 1 or st[0] >= (r - 1) * st[1] + c, "matrices overlap", t.shape, st)
+        return t.data_ptr(), st[0] if len(st) == 3 else 0, max(st[-2], c)
+
+    def run(self):
+        if not self.out:
+            return self.out
+        with _on(self._dev):
+            ws = torch.empty((self._need,), dtype=torch.uint8, device=self._dev)
+            check(_lib.load().dino_ortho(self._items, len(self.out), self._steps, self._coeffs, self._eps, ws.data_ptr(),
+                                         self._need, _stream()), "dino_ortho")
+        return self.out
+
+
 def orthogonalize(updates, *, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
     """Orthogonalised updates by Newton-Schulz products (include/dino_hip.h: dino_ortho), all matrices in one sequence of
     launches.  updates: a tensor or a list of tensors, each [rows, cols] or [batch, rows, cols] in fp32 / bf16, columns
     side by side, rows with any stride.  coeffs: (a, b, c), or one such triple per step.  Returns bf16 tensors of the same
     shapes (a tensor for a tensor, a list for a list); out: the caller's own, in the same form."""
-    single = isinstance(updates, torch.Tensor)
-    ups = [updates] if single else list(updates)
-    _req(isinstance(steps, int) and 1 <= steps <= ORTHO_MAX_STEPS, f"steps: 1 to {ORTHO_MAX_STEPS}", steps)
-    rows = [tuple(c) for c in coeffs] if len(coeffs) and not isinstance(coeffs[0], (int, float)) else [tuple(coeffs)] * steps
-    _req(len(rows) == steps and all(len(c) == 3 for c in rows), "coeffs: (a, b, c), or one triple per step", coeffs)
-    _req(isinstance(eps, (int, float)) and 0.0 <= eps < 1e30, "eps", eps)
-    if not ups:
-        return []
-    outs = [None] * len(ups) if out is None else ([out] if single else list(out))
-    _req(len(outs) == len(ups), "out: one for each update")
-    _dev(*ups, *outs)
-    dev = ups[0].device
-    items = (_lib.OrthoItem * len(ups))()
-    res = []
-    with _on(dev):
-        for q, u, o in zip(items, ups, outs):
-            _req(u.dim() in (2, 3) and u.device == dev, "updates: [rows, cols] or [batch, rows, cols] on one device", u.shape)
-            if o is None:
-                o = torch.empty(u.shape, dtype=torch.bfloat16, device=dev)
-            _req(o.shape == u.shape and o.dtype is torch.bfloat16 and o.device == dev, "out: bf16 of the update's shape")
-            r, c = u.shape[-2:]
-            for t in (u, o):
-                _req(r > 0 and c > 0 and (t.stride(-1) == 1 or c == 1) and (t.stride(-2) >= c or r == 1),
-                     "columns side by side, rows apart", t.shape, t.stride())
-                _req(t.dim() == 2 or t.shape[0] <= 1 or t.stride(0) >= (r - 1) * t.stride(1) + c, "matrices overlap", t.stride())
-            q.inp, q.out = u.data_ptr(), o.data_ptr()
-            q.rows, q.cols, q.dtype = r, c, dt_code(u.dtype)
-            q.in_ld, q.out_ld = max(u.stride(-2), c), max(o.stride(-2), c)
-            if u.dim() == 3:
-                q.batch, q.in_batch, q.out_batch = u.shape[0], u.stride(0), o.stride(0)
-            else:
-                q.batch = 1
-            res.append(o)
-        cf = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
-        need = ctypes.c_int64(0)
-        lib = _lib.load()
-        check(lib.dino_ortho_workspace(items, len(ups), ctypes.byref(need)), "dino_ortho_workspace")
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
-        check(lib.dino_ortho(items, len(ups), steps, cf, float(eps), ws.data_ptr(), need.value, _stream()), "dino_ortho")
-    return res[0] if single else res
+    if isinstance(updates, torch.Tensor):
+        return OrthoPlan([updates], None if out is None else [out], steps=steps, coeffs=coeffs, eps=eps).run()[0]
+    return OrthoPlan(updates, out, steps=steps, coeffs=coeffs, eps=eps).run()
+
+
+def muon_momentum(grad, momentum, update, chunks, hp, coef, mu, nesterov):
+    """One pass over the chunks of Muon's matrices (include/dino_hip.h: dino_muon_momentum)."""
+    _dev(grad, momentum, update, chunks, hp, coef)
+    _f32(grad, momentum, update, hp, coef)
+    _req(grad.numel() == momentum.numel() == update.numel())
+    _req(chunks.dtype == torch.int64 and chunks.is_contiguous() and chunks.dim() == 2 and chunks.shape[1] == 3)
+    _req(hp.dim() == 2 and hp.shape[1] == 8 and (coef is None or coef.numel() >= hp.shape[0]))
+    check(_lib.load().dino_muon_momentum(_p(grad), _p(momentum), _p(update), _p(chunks), chunks.shape[0], _p(hp),
+                                         _p(coef), float(mu), int(bool(nesterov)), _stream()), "dino_muon_momentum")
+
+
+def muon_apply(param, ortho, chunks, hp):
+    """param = param (1 - lr wd) - lr scale ortho over the chunks (include/dino_hip.h: dino_muon_apply)."""
+    _dev(param, ortho, chunks, hp)
+    _f32(param, hp)
+    _req(ortho.dtype == torch.bfloat16 and ortho.is_contiguous() and ortho.numel() == param.numel())
+    _req(chunks.dtype == torch.int64 and chunks.is_contiguous() and chunks.dim() == 2 and chunks.shape[1] == 3)
+    _req(hp.dim() == 2 and hp.shape[1] == 8)
+    check(_lib.load().dino_muon_apply(_p(param), _p(ortho), _p(chunks), chunks.shape[0], _p(hp), _stream()),
+          "dino_muon_apply")
 
 
 def ema(teacher, student, teacher_shadow, m, one_minus_m):

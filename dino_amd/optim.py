@@ -1,9 +1,14 @@
-"""FusedAdamW: torch.optim.AdamW semantics (reference dino.py:251, train_utils.py:56-59,131)
+"""FusedAdamW and FusedMuon over the student's flat parameter buffer.
+
+FusedAdamW: torch.optim.AdamW semantics (reference dino.py:251, train_utils.py:56-59,131)
 as ONE streaming kernel over the student's flat parameter buffer, fused with the per-tensor
 gradient clip factor, the momentum-teacher EMA (train_utils.py:152-162) and the refresh of
 the bf16 weight shadows of student and teacher.
 
-It subclasses torch.optim.Optimizer so param_groups / state_dict keep the reference's shape
+FusedMuon: the hidden matrices by orthogonalised momentum (all of them in one sequence of launches), everything else by
+the same AdamW pass, which also does the EMA and the shadows of both.
+
+They subclass torch.optim.Optimizer so param_groups / state_dict keep the reference's shape
 (the step loop rewrites param_groups[i]["lr"/"weight_decay"] every iteration).
 """
 import time
@@ -122,6 +127,7 @@ class FusedAdamW(torch.optim.Optimizer):
             b1, b2 = group["betas"]
             # torch skips a parameter without a gradient: no moment update, no decay, no step count
             active = np.fromiter((p.grad is not None for p in params), dtype=bool, count=len(params))
+            active = self._split_off(group, rows, active, hp)
             r = rows[active]
             self._steps[r] += 1
             t = self._steps[r]
@@ -142,6 +148,7 @@ class FusedAdamW(torch.optim.Optimizer):
             if tst.layout.total != st.layout.total:
                 raise ValueError("teacher and student layouts differ")
             m = float(ema_momentum)
+        self._before_adamw(st, clip_coef)
         ops.adamw_ema(st.flat, st.grad_flat, self.exp_avg, self.exp_avg_sq,
                       None if tst is None else tst.flat,
                       st.shadow if st.bf16 else None,
@@ -153,6 +160,13 @@ class FusedAdamW(torch.optim.Optimizer):
             tst.refresh_derived()
         return None
 
+    def _split_off(self, group, rows, active, hp):
+        """Which of a group's rows AdamW updates (a subclass takes some for itself and fills their hp rows)."""
+        return active
+
+    def _before_adamw(self, st, clip_coef):
+        """Updates of the rows that _split_off took; AdamW's pass then does their EMA and shadows."""
+
     def zero_grad(self, set_to_none: bool = True):
         st = self._bind()
         if set_to_none:
@@ -160,6 +174,80 @@ class FusedAdamW(torch.optim.Optimizer):
                 p.grad = None
         st.grad_flat.zero_()
         st._need_zero = False
+
+
+class FusedMuon(FusedAdamW):
+    """Muon for the hidden matrices of the backbone's blocks and the head's MLP (2-D weights; qkv as three matrices),
+    AdamW for everything else -- embeddings, norms, biases, the prototypes -- in one step() with FusedAdamW's contract.
+
+        buf = momentum * buf + grad;  u = grad + momentum * buf  (nesterov) or buf
+        weight = weight * (1 - lr * weight_decay) - lr * scale * orthogonalize(u)
+
+    scale: "rms" = 0.2 * sqrt(max(rows, cols)), which gives the update the size of AdamW's, so one learning-rate schedule
+    serves both; "spectral" = sqrt(max(1, rows / cols)).  select(name, parameter) -> bool chooses the matrices.
+    state[p]["exp_avg"] of a matrix is its momentum buffer (and its "exp_avg_sq" stays zero): checkpoints keep AdamW's
+    layout."""
+
+    def __init__(self, params, student, teacher=None, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+                 momentum=0.95, nesterov=True, ns_steps=5, ns_coeffs=ops.NS_COEFFS, ns_eps=1e-7, scale="rms", select=None):
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"FusedMuon: momentum {momentum} is not in [0, 1)")
+        if scale not in ("rms", "spectral"):
+            raise ValueError(f"FusedMuon: scale is \"rms\" or \"spectral\", got {scale!r}")
+        super().__init__(params, student, teacher, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+        self.momentum, self.nesterov = float(momentum), bool(nesterov)
+        self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, float(ns_eps)
+        self.scale, self._select = scale, select if select is not None else is_hidden_matrix
+
+    def _bind(self):
+        old = self._st
+        st = super()._bind()
+        if st is not old:
+            names = [k for k in st.layout.names if st.params[k].requires_grad and self._select(k, st.params[k])]
+            for k in names:
+                if st.params[k].dim() != 2:
+                    raise ValueError(f"FusedMuon: {k} is not a matrix")
+            index = {k: i for i, k in enumerate(st.layout.names)}
+            mine = set(index[k] for k in names)
+            keep = torch.tensor([int(t) in mine for t in st.layout.chunks[:, 0]], dtype=torch.bool)
+            self._mchunks = st.layout.chunks[keep].contiguous().to(st.device)
+            self._update = torch.zeros(st.layout.total, dtype=torch.float32, device=st.device)
+            self._ortho = torch.zeros(st.layout.total, dtype=torch.bfloat16, device=st.device)
+            self._mscale = np.zeros(len(st.layout.names))
+            mats = []                                 # (update, ortho) views
+            for k in names:
+                r, c = st.params[k].shape
+                parts = 3 if k.endswith("attn.qkv.weight") and r == 3 * c else 1
+                rr = r // parts
+                self._mscale[index[k]] = 0.2 * max(rr, c) ** 0.5 if self.scale == "rms" else max(1.0, rr / c) ** 0.5
+                shape = (parts, rr, c)
+                mats.append((st.layout.view(self._update, k).view(shape), st.layout.view(self._ortho, k).view(shape)))
+            self._plan = ops.OrthoPlan([u for u, _ in mats], [o for _, o in mats], steps=self.ns_steps,
+                                       coeffs=self.ns_coeffs, eps=self.ns_eps)
+        return st
+
+    def _split_off(self, group, rows, active, hp):
+        mine = self._mscale[rows] != 0
+        take = rows[mine & active]
+        hp[take, 0], hp[take, 1] = group["lr"], group["weight_decay"]
+        hp[take, 5], hp[take, 6] = 1.0, self._mscale[take]
+        self._steps[take] += 1
+        return active & ~mine
+
+    def _before_adamw(self, st, clip_coef):
+        if not self._plan.out:
+            return
+        ops.muon_momentum(st.grad_flat, self.exp_avg, self._update, self._mchunks, self._hp_dev, clip_coef,
+                          self.momentum, self.nesterov)
+        self._plan.run()
+        ops.muon_apply(st.flat, self._ortho, self._mchunks, self._hp_dev)
+
+
+def is_hidden_matrix(name, param):
+    """The weights that act on hidden features: linear layers of the blocks and of the head's MLP (not the patch or
+    position embeddings, norms, biases, or the prototypes)."""
+    return (param.dim() == 2 and name.endswith(".weight")
+            and ("blocks." in name or ".mlp" in "." + name) and "last_layer" not in name)
 
 
 @torch.no_grad()

@@ -20,9 +20,10 @@ from .utils import cancel_gradients_last_layer, grad_stats_async
 _TEACHER_STREAM = os.environ.get("DINO_TEACHER_STREAM", "1") != "0"
 
 def train_step(student, teacher, dino_loss, optimizer, images, iteration, lr_schedule, wd_schedule,
-               momentum_schedule, clip_grad, freeze_last_layer_iter, sync_stats=False):
+               momentum_schedule, clip_grad, freeze_last_layer_iter, sync_stats=False, watch=None):
     """One step on device-resident `images` (list of crops).  Returns (loss tensor, stats work).
-    No host synchronisation unless sync_stats."""
+    No host synchronisation unless sync_stats.  watch: a dict to fill with DINOLoss.watch's values (entropies, agreement)
+    of this step's outputs; it costs one more pass over the logits and changes no result."""
     for i, group in enumerate(optimizer.param_groups):          # train_utils.py:56-59
         group["lr"] = float(lr_schedule[iteration])          # plain floats: the optimizer state_dict
         if i == 0:                                            # stays loadable with weights_only=True
@@ -41,6 +42,8 @@ def train_step(student, teacher, dino_loss, optimizer, images, iteration, lr_sch
         with torch.no_grad():
             teacher_output = teacher(images[:2])                      # :75-77
         student_output = student(images)                              # :85
+    if watch is not None:
+        watch.update(dino_loss.watch(student_output, teacher_output, iteration))
     loss = dino_loss(student_output, teacher_output, iteration)   # :87
     optimizer.zero_grad()                                         # :115
     loss.backward()                                               # :118 (+ flat-bucket all-reduce)
@@ -61,9 +64,11 @@ def train_one_epoch(student, teacher, teacher_without_ddp, dino_loss, data_loade
                     lr_schedule, wd_schedule, momentum_schedule, epoch, nepochs, fp16_scaler,
                     clip_grad, freeze_last_layer_iter, save_every, checkpoint_dir, gpu_id,
                     domain_classifier=None, domain_loss_fn=None, grl=None, dc_clip_grad: float = 0,
-                    log_every: int = 50):
+                    log_every: int = 50, watch_every: int = 0):
     """Reference signature (train_utils.py:14-36).  fp16_scaler is accepted and ignored: the
-    bf16 path needs no loss scaling.  The adversarial branch is out of scope."""
+    bf16 path needs no loss scaling.  The adversarial branch is out of scope.
+    watch_every > 0: every so many steps DINOLoss.watch is taken too, and its averages over them join the returned
+    stats."""
     if domain_classifier is not None:
         raise NotImplementedError("domain-adversarial branch (adversarial.enable) is out of scope")
     if distributed.is_enabled() and hasattr(data_loader, "sampler") and hasattr(data_loader.sampler, "set_epoch"):
@@ -71,6 +76,7 @@ def train_one_epoch(student, teacher, teacher_without_ddp, dino_loss, data_loade
     device = torch.device("cuda" if gpu_id == -1 else f"cuda:{gpu_id}")
     loss_sum = torch.zeros((), dtype=torch.float32, device=device)
     n = 0
+    nwatch, watched = 0, {}
     last = None
     from ..data import CropPrefetcher
     # host -> HBM two batches ahead on a copy stream (the reference copies at the top of the step,
@@ -78,9 +84,13 @@ def train_one_epoch(student, teacher, teacher_without_ddp, dino_loss, data_loade
     feed = data_loader if isinstance(data_loader, CropPrefetcher) else CropPrefetcher(data_loader, device)
     for it, (images, _labels) in enumerate(feed):
         iteration = len(data_loader) * epoch + it
+        seen = {} if watch_every and it % watch_every == 0 else None
         loss, _ = train_step(student, teacher_without_ddp, dino_loss, optimizer, images, iteration,
                              lr_schedule, wd_schedule, momentum_schedule, clip_grad,
-                             freeze_last_layer_iter)
+                             freeze_last_layer_iter, watch=seen)
+        if seen is not None:
+            nwatch += 1
+            watched = {k: v + watched[k] if k in watched else v for k, v in seen.items()}
         loss_sum += loss.detach()
         n += 1
         last = loss
@@ -104,10 +114,14 @@ def train_one_epoch(student, teacher, teacher_without_ddp, dino_loss, data_loade
     # global averages, as the reference's MetricLogger.synchronize_between_processes (:191): the loss
     # is averaged over the steps of every rank; lr / wd are the last step's values (the reference's
     # meters average them over the epoch -- they are schedule values, identical on all ranks)
-    tot = torch.stack([loss_sum.double(), torch.tensor(float(n), dtype=torch.float64, device=device)])
+    tot = torch.stack([loss_sum.double(), torch.tensor(float(n), dtype=torch.float64, device=device)]
+                      + [watched[k].double() for k in sorted(watched)]
+                      + ([torch.tensor(float(nwatch), dtype=torch.float64, device=device)] if watched else []))
     if distributed.is_enabled_and_multiple_gpus():
         distributed.all_reduce(tot)
     tot = tot.tolist()
     stats = {"loss": tot[0] / max(tot[1], 1.0), "lr": optimizer.param_groups[0]["lr"],
              "wd": optimizer.param_groups[0]["weight_decay"]}
+    for k, v in zip(sorted(watched), tot[2:]):
+        stats[k] = v / tot[-1]
     return stats

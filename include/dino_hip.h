@@ -328,6 +328,14 @@ typedef struct dino_ortho_item {
 int dino_ortho_workspace(const dino_ortho_item* items /* host */, int count, int64_t* bytes /* host */);
 int dino_ortho(const dino_ortho_item* items /* host */, int count, int steps, const float* coeffs /* host, 3 * steps */,
                double eps, void* workspace, int64_t workspace_bytes, void* stream);
+/* Muon's passes around dino_ortho over the flat buffers (chunks: those of its matrices only; hp as for dino_adamw_ema with
+ * hp[5] = 1 where the tensor takes part -- it has a gradient -- else 0, hp[6] = the factor of its update):
+ *   momentum = mu * momentum + coef[tensor] * grad,   update = nesterov ? coef * grad + mu * momentum : momentum
+ *   param = param * (1 - lr * weight_decay) - lr * hp[6] * ortho     (ortho: bf16, at the parameters' offsets)
+ * dino_adamw_ema with the tensor inactive then forms its EMA and shadows. */
+int dino_muon_momentum(const float* grad, float* momentum, float* update, const int64_t* chunks, int nchunks,
+                       const float* hp, const float* coef, float mu, int nesterov, void* stream);
+int dino_muon_apply(float* param, const void* ortho, const int64_t* chunks, int nchunks, const float* hp, void* stream);
 /* stand-alone EMA over a flat range (same reference lines) + optional shadow refresh */
 int dino_ema(float* teacher, const float* student, void* teacher_shadow, int64_t n, float m,
              float one_minus_m, void* stream);
