@@ -288,6 +288,21 @@ DEVI void dma16(unsigned lds, int voff, const u32x4& rs, int soff) {
 // transposing read touches lie in different banks
 DEVI int tkey(int row) { return 2 * ((row >> 3) & 1); }
 
+// odd rows of 16 lanes of w[0], w[1] trade places with even rows of w[2], w[3] (its own inverse)
+DEVI u32x4 swap16(const u32x4& w) {
+    const auto x = __builtin_amdgcn_permlane16_swap(w[0], w[2], false, false);
+    const auto y = __builtin_amdgcn_permlane16_swap(w[1], w[3], false, false);
+    return u32x4{x[0], y[0], x[1], y[1]};
+}
+// eight 16-bit values, of which `left` lie inside the row
+DEVI void store8x16(uint16_t* o, const u32x4& w, bool aligned, int left) {
+    if (aligned && left >= 8) *(u32x4*)o = w;
+    else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) o[k] = (uint16_t)(k & 1 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu);
+    }
+}
 template <bool TOBF> DEVI unsigned pack2(float a, float b) {
     if (TOBF) {
         const bf16x2 v = {(bf16)a, (bf16)b};
@@ -444,11 +459,11 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         const int nend = SYM ? mp : np;
         // where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 64, so a
         // fragment is inside as a whole or outside as a whole)
-        const int vlane = i * 64 + g * 8;
-        auto upart = [&](int ni) {           // (+ 1024 mi)
-            const int n = wn0 + 16 * ni;
-            return ((n >> 5) * mp + wm0) * 64 + (n & 31) * 2;
-        };
+        // A store or load takes 16 bytes a lane: the two fragments of a panel trade halves between lanes 16 apart, after
+        // which lane (i, g) holds columns 8 (g / 2) .. + 7 of fragment ni + g % 2 -- 64 bytes of a row from four lanes,
+        // 1 KB in one piece from the wave.
+        const int vlane = i * 64 + (g & 1) * 32 + (g >> 1) * 16;
+        auto upart = [&](int ni) { return (((wn0 + 16 * ni) >> 5) * mp + wm0) * 64; };     // (ni even; + 1024 mi)
         if (MODE == POLY) {
             // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads a neighbour or
             // zero and is not stored)
@@ -456,19 +471,24 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
             constexpr int PART = MI / 2;
 #pragma unroll
             for (int q = 0; q < MI; q += PART) {
-                f16x4 el[PART][NI];
+                u32x4 el[PART][NI / 2];
 #pragma unroll
                 for (int mi = 0; mi < PART; ++mi)
 #pragma unroll
-                    for (int ni = 0; ni < NI; ++ni)
-                        el[mi][ni] = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rs, vlane + (q + mi) * 1024, upart(ni), 0));
+                    for (int ni = 0; ni < NI; ni += 2)
+                        el[mi][ni / 2] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, vlane + (q + mi) * 1024, upart(ni), 0));
 #pragma unroll
                 for (int mi = 0; mi < PART; ++mi)
 #pragma unroll
-                    for (int ni = 0; ni < NI; ++ni)
+                    for (int ni = 0; ni < NI; ni += 2) {
+                        const u32x4 w = swap16(el[mi][ni / 2]);
+                        const f16x4 x0 = __builtin_bit_cast(f16x4, u32x2{w[0], w[1]}), x1 = __builtin_bit_cast(f16x4, u32x2{w[2], w[3]});
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            acc[q + mi][ni][r] = fmaf(c0, (float)el[mi][ni][r], acc[q + mi][ni][r] * c1);
+                        for (int r = 0; r < 4; ++r) {
+                            acc[q + mi][ni][r] = fmaf(c0, (float)x0[r], acc[q + mi][ni][r] * c1);
+                            acc[q + mi][ni + 1][r] = fmaf(c0, (float)x1[r], acc[q + mi][ni + 1][r] * c1);
+                        }
+                    }
             }
             if (d.m0 == d.n0) {
                 int off = wm0 + i - wn0 - 4 * g;
@@ -488,18 +508,21 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[mi][ni][r] *= c1;
         }
-        // fp16 results go to panels: 32 bytes of 16 rows a store
+        // the fragments (mi, ni) and (mi, ni + 1) as 16 bytes a lane
+        auto pair = [&](auto tobf_c, int mi, int ni) {
+            constexpr bool TOBF = decltype(tobf_c)::value;
+            const f32x4 a = acc[mi][ni], b = acc[mi][ni + 1];
+            return swap16(u32x4{pack2<TOBF>(a[0], a[1]), pack2<TOBF>(a[2], a[3]), pack2<TOBF>(b[0], b[1]), pack2<TOBF>(b[2], b[3])});
+        };
         auto put = [&](f16* dst) {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)dst, 0, mp * nend * 2, 0x00020000);
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) {
+            for (int ni = 0; ni < NI; ni += 2) {
                 if (wn0 + 16 * ni >= nend) continue;
 #pragma unroll
                 for (int mi = 0; mi < MI; ++mi) {
                     if (wm0 + 16 * mi >= mp) continue;
-                    const f32x4 v = acc[mi][ni];
-                    __builtin_amdgcn_raw_buffer_store_b64(u32x2{pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3])}, rs,
-                                                          vlane + mi * 1024, upart(ni), 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(pair(std::false_type{}, mi, ni), rs, vlane + mi * 1024, upart(ni), 0);
                 }
             }
         };
@@ -521,21 +544,15 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                     *(unsigned*)(img + at(c, m)) = odd ? pack2<TOBF>(x0, v[2]) : pack2<TOBF>(v[0], x0);
                     *(unsigned*)(img + at(c + 1, m)) = odd ? pack2<TOBF>(x1, v[3]) : pack2<TOBF>(v[1], x1);
                 }
-                for (int e = lane; e < 4 * C::SUBM; e += 64) {
+                for (int e = lane; e < 2 * C::SUBM; e += 64) {
                     // panels: 64 bytes of each of the 16 columns; else whole columns
-                    const int c = TOBF ? e / (C::SUBM / 4) : (e >> 3) & 15;
-                    const int m = TOBF ? (e - c * (C::SUBM / 4)) * 4 : (e >> 7) * 32 + (e & 7) * 4;
-                    const u32x2 w = *(const u32x2*)(img + at(c, m));
+                    const int c = TOBF ? e / (C::SUBM / 8) : (e >> 2) & 15;
+                    const int m = TOBF ? (e - c * (C::SUBM / 8)) * 8 : (e >> 6) * 32 + (e & 3) * 8;
+                    const u32x4 w = *(const u32x4*)(img + at(c, m));
                     const int dr = wn0 + ni * 16 + c, dc = wm0 + m;
                     if (dr >= rows || dc >= cols) continue;
                     uint16_t* o = dst + (TOBF ? dr * ld + dc : ((int64_t)(dc >> 5) * ld + dr) * 32 + (dc & 31));
-                    if (!TOBF || (aligned && dc + 4 <= cols)) *(u32x2*)o = w;
-                    else {
-                        const unsigned x[4] = {w[0] & 0xffffu, w[0] >> 16, w[1] & 0xffffu, w[1] >> 16};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (dc + k < cols) o[k] = (uint16_t)x[k];
-                    }
+                    store8x16(o, w, !TOBF || aligned, cols - dc);
                 }
             }
         };
@@ -560,24 +577,17 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         } else {
             const Mat& q = ws.mats[d.item];
             bf16* out = (bf16*)q.out + d.mat * q.out_batch;
-            const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 7) == 0;
+            const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 15) == 0;
             if (q.tall) put_columns(std::true_type{}, (uint16_t*)out, q.out_ld, q.n, q.m, al);
             else {
 #pragma unroll
                 for (int mi = 0; mi < MI; ++mi) {
                     const int m = wm0 + mi * 16 + i;
-                    if (m >= q.m) continue;
 #pragma unroll
-                    for (int ni = 0; ni < NI; ++ni) {
-                        const int n = wn0 + 16 * ni + 4 * g;
-                        const f32x4 v = acc[mi][ni];
-                        bf16* o = out + m * q.out_ld + n;
-                        if (al && n + 4 <= q.n) *(u32x2*)o = u32x2{pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3])};
-                        else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (n + r < q.n) o[r] = (bf16)v[r];
-                        }
+                    for (int ni = 0; ni < NI; ni += 2) {
+                        const u32x4 w = pair(std::true_type{}, mi, ni);
+                        const int n = wn0 + 16 * ni + (g & 1) * 16 + (g >> 1) * 8;
+                        if (m < q.m && n < q.n) store8x16((uint16_t*)out + m * q.out_ld + n, w, al, q.n - n);
                     }
                 }
             }
