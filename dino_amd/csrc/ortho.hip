@@ -250,8 +250,10 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 // (a on B's diagonal instead of a X in the update: no second read of X.)
 // Operands go global -> LDS by DMA in a ring of S stages of 32 along the contraction, one stream of stages over all tiles of
 // the workgroup: the next tile's first stages are on their way while this one's results leave.  With SPLIT (an UPDATE) a
-// stage holds the hi and the lo part of X and feeds two products.  The path from L2 to the CUs bounds these products (about
-// 9.4 TB/s: T / 2 operations a byte), hence the large tiles.
+// stage holds the hi and the lo part of X and feeds two products.
+// What bounds it, for X' of ViT-L's 144 matrices (0.62 TFLOP; 0.9 GB to read, 0.6 GB to write): 610 us = 1010 TFLOP/s (a large
+// library product reaches 1306 here).  Alone, the requests take 329 us, the products 282, reading fragments and products
+// 390, all but writing the results 442: no single one bounds it, the phases do not overlap them fully.
 // The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
 // multiplies.  Waves 4..7 ("late") run one phase behind waves 0..3: stage s is read in phases 2s and 2s + 1, its slot is
 // refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.
@@ -294,10 +296,13 @@ DEVI u32x4 swap16(const u32x4& w) {
     const auto y = __builtin_amdgcn_permlane16_swap(w[1], w[3], false, false);
     return u32x4{x[0], y[0], x[1], y[1]};
 }
-// eight 16-bit values, of which `left` lie inside the row
-DEVI void store8x16(uint16_t* o, const u32x4& w, bool aligned, int left) {
-    if (aligned && left >= 8) *(u32x4*)o = w;
-    else {
+// eight 16-bit values, of which `left` lie inside the row; addresses are multiples of `align` bytes
+DEVI void store8x16(uint16_t* o, const u32x4& w, int align, int left) {
+    if (align >= 16 && left >= 8) *(u32x4*)o = w;
+    else if (align >= 8 && left >= 8) {
+        *(u32x2*)o = u32x2{w[0], w[1]};
+        *(u32x2*)(o + 4) = u32x2{w[2], w[3]};
+    } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (k < left) o[k] = (uint16_t)(k & 1 ? w[k / 2] >> 16 : w[k / 2] & 0xffffu);
@@ -333,8 +338,9 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     // ---- stages: 32 columns of T rows of P ([row][4 chunks of 16 B]), and of Q either the same or, for UPDATE, 32 rows
     // of T columns (T / 32 panels of [32 rows][4 chunks]).  The operands lie in memory as panels of 32 columns, so every
     // DMA of a wave moves 1 KB in one piece.  Chunks are permuted by a key of the row so that no read meets itself
-    // in a bank.  Rows and columns behind the matrix read zeros or neighbours: only their own results, which are not
-    // stored, see them.  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
+    // in a bank.  Rows behind the matrix read zeros or the next panel, panels behind it the last one: only their own
+    // results, which are not stored, see them.  (A request never starts behind its buffer: the range check subtracts the
+    // uniform part of the offset from the size.)  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
     int voP[ND], voQ[ND];
 #pragma unroll
     for (int u = 0; u < ND; ++u) {
@@ -344,12 +350,13 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
     }
     u32x4 rsP, rsQ[SPLIT ? 2 : 1];
     const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
-    int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, islot = 0, issued = 0;
+    int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, ilast = 0, islot = 0, issued = 0;
     Tile tn = load_tile(tiles + b0);                       // the tile after the one being requested
     auto open = [&]() {                        // start requesting tile tn
         imp = tn.mp;
         im0 = tn.m0;
         in0 = tn.n0;
+        ilast = (tn.np >> 5) - 1;
         itotal = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
         rsP = rsrc(MODE == GRAM ? ws.x[ga.src][0] + tn.xo : MODE == POLY ? ws.a + tn.ao : ws.b + tn.ao,
                    tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
@@ -372,7 +379,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
                 for (int u = 0; u < ND; ++u) {
                     const int kp = SPLIT ? ik : ik * KB + h;   // panel along the contraction
-                    const int so = SYM ? (kp * imp + in0) * 64 : (((in0 >> 5) + ((wave + 8 * u) >> 1)) * imp + kp * 32) * 64;
+                    const int so = SYM ? (kp * imp + in0) * 64 : (min((in0 >> 5) + ((wave + 8 * u) >> 1), ilast) * imp + kp * 32) * 64;
                     dma16(at + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h : 0], so);
                 }
             ++issued;
@@ -457,15 +464,16 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         const float c0 = ga.c0 * e2, c1 = MODE == POLY ? ga.c1 * e2 * e2 : MODE == FINAL ? ga.c1 * e1 : ga.c1;
         const int wm0 = d.m0 + wm * C::SUBM, wn0 = d.n0 + wn * C::SUBN;
         const int nend = SYM ? mp : np;
-        // where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 64, so a
-        // fragment is inside as a whole or outside as a whole)
+        // Where fragment (mi, ni) lies in a matrix of panels: a lane's part and a uniform one (mp is a multiple of 64, so a
+        // fragment is inside as a whole or outside as a whole).
         // A store or load takes 16 bytes a lane: the two fragments of a panel trade halves between lanes 16 apart, after
         // which lane (i, g) holds columns 8 (g / 2) .. + 7 of fragment ni + g % 2 -- 64 bytes of a row from four lanes,
         // 1 KB in one piece from the wave.
         const int vlane = i * 64 + (g & 1) * 32 + (g >> 1) * 16;
-        auto upart = [&](int ni) { return (((wn0 + 16 * ni) >> 5) * mp + wm0) * 64; };     // (ni even; + 1024 mi)
+        auto upart = [&](int ni) { return (min((wn0 + 16 * ni) >> 5, (nend >> 5) - 1) * mp + min(wm0, mp - 16)) * 64; };
+        // (ni even; + 1024 mi)
         if (MODE == POLY) {
-            // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads a neighbour or
+            // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads another one or
             // zero and is not stored)
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a + d.ao), 0, mp * mp * 2, 0x00020000);
             constexpr int PART = MI / 2;
@@ -528,7 +536,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         };
         // ... by columns (a mirrored tile, a tall matrix of the caller's) through an image of 16 columns at a time in LDS, so
         // that a store covers rows of the destination; a wave reads only what it wrote.
-        auto put_columns = [&](auto tobf_c, uint16_t* dst, int64_t ld, int rows, int cols, bool aligned) {
+        auto put_columns = [&](auto tobf_c, uint16_t* dst, int64_t ld, int rows, int cols, int align) {
             constexpr bool TOBF = decltype(tobf_c)::value;
             constexpr int RB = C::SUBM * 2;
             auto at = [&](int c, int m) { return c * RB + ((m * 2) ^ ((c >> 1 & (C::SUBM / 16 - 1)) << 5)); };
@@ -552,7 +560,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
                     const int dr = wn0 + ni * 16 + c, dc = wm0 + m;
                     if (dr >= rows || dc >= cols) continue;
                     uint16_t* o = dst + (TOBF ? dr * ld + dc : ((int64_t)(dc >> 5) * ld + dr) * 32 + (dc & 31));
-                    store8x16(o, w, !TOBF || aligned, cols - dc);
+                    store8x16(o, w, TOBF ? align : 16, cols - dc);
                 }
             }
         };
@@ -567,7 +575,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         if (SYM) {
             f16* o = (MODE == GRAM ? ws.a : ws.b) + d.ao;
             put(o);
-            if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)o, mp, mp, mp, true);
+            if (d.m0 != d.n0) put_columns(std::false_type{}, (uint16_t*)o, mp, mp, mp, 16);
         } else if (MODE == UPDATE) {
             put(ws.x[ga.src ^ 1][0] + d.xo);
             if (SPLIT && ga.split_next) {          // (pairs are used from the first step on)
@@ -577,7 +585,8 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
         } else {
             const Mat& q = ws.mats[d.item];
             bf16* out = (bf16*)q.out + d.mat * q.out_batch;
-            const bool al = (((uintptr_t)out | (uint64_t)(q.out_ld * 2)) & 15) == 0;
+            const uint64_t bits = (uintptr_t)out | (uint64_t)(q.out_ld * 2);
+            const int al = (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : 2;
             if (q.tall) put_columns(std::true_type{}, (uint16_t*)out, q.out_ld, q.n, q.m, al);
             else {
 #pragma unroll
@@ -671,8 +680,9 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         if (out) out[i] = q;
     }
     // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
-    // the CUs, a tile costing its operands' way from L2 (T a stage); of the smaller ones two share a CU, and what one
-    // starts and ends with overlaps the other: 0.65.
+    // the 256 CUs, a tile of 256 costing 256 a stage and one of 128, two of which share a CU and overlap their starts and
+    // ends, 83.  Measured, 256 against 128 (us, per launch): ViT-L's matrices (1440 / 5184 tiles) A 416 / 491, B 287 / 335,
+    // X' 650 / 889; ViT-S's (216 / 432) A 52 / 35, B 28 / 18, X' 36 / 35; 2048 x 2048 and the head's A 61 / 33, X' 57 / 46.
     for (int kind = 0; kind < 2; ++kind) {
         double best = 0;
         for (int T = 256; T >= 128; T /= 2) {
@@ -689,8 +699,6 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
             const double cost = work / tiles * ceil(tiles / 256) * (T == 256 ? 256 : 83);
             if (T == 256 || cost < best) { best = cost; L.tile[kind] = T; }
         }
-        static const char* force[2] = {getenv("OT_SYM"), getenv("OT_RECT")};
-        if (force[kind]) L.tile[kind] = atoi(force[kind]);
     }
     // tiles with the longest contraction first: the last round then ends evenly
     int* order = (int*)malloc(sizeof(int) * (size_t)(count + 1));
@@ -738,10 +746,16 @@ void poly_bounds(const float* c, double top, double& px, double& qx) {
 
 template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStream_t st) {
     constexpr int smem = Cfg<T, SPLIT>::SMEM;
-    static const hipError_t set = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>,
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (set != hipSuccess) return (int)set;
-        const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
+    static bool ready[64];                            // by device; two threads may both set it, to the same
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        e = hipFuncSetAttribute((const void*)ortho_gemm_kernel<MODE, T, SPLIT>, hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != hipSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
     hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3(ga.ntiles < most ? ga.ntiles : most), dim3(512), smem, st, ga);
     return dino_launch_status();
 }

@@ -16,11 +16,12 @@ SPLIT_ABOVE = 16.0
 def recurrence(u, steps=5, coeffs=NS, eps=1e-7):
     """(result, tolerance) in 64 bits on the CPU.  The tolerance is on the Frobenius norm of the difference.
 
-    A step's operands X, A, B are rounded to fp16 (half a step: 2^-11 of an element; 2^-22 as hi + lo pairs, which they
-    are while the growth is above 16), so a step adds an error of about three times rms(rounding) |X|_F, with rms = half /
-    sqrt(3), that the later steps multiply by at most the product of their a (derivative at 0, the largest).
+    A step rounds X, A and B to fp16 (half a step: 2^-11 of an element).  X's rounding is multiplied by the later steps, by
+    at most the product of their a (derivative at 0, the largest); while that is above 8 X is a pair of fp16 (2^-22), so the
+    limit of 16 below allows more than is used.  A's and B's multiply X from the left and stay relative to it.  Counted here:
+    three roundings of rms half / sqrt(3) a step, all growing, of a whole fp16 from a growth of 16 down, of 2^-20 before.
     Independent roundings add in squares; three times that is allowed.  The bf16 result adds half a step, 2^-8, of itself.
-    fp32 sums of K terms stay below 2^-24 sqrt(K), less than the pairs' 2^-22 for the sizes here times 4."""
+    fp32 sums of K terms stay below 2^-24 sqrt(K), less than 2^-20 for the sizes here."""
     x = u.double()
     x = x / (torch.linalg.vector_norm(x) + eps)
     tall = x.shape[0] > x.shape[1]
@@ -83,6 +84,22 @@ def test_many_items_in_one_call():
             off(b, a)
     again = ops.orthogonalize([u.cuda() for u in ups])
     assert all(torch.equal(a, b) for a, b in zip(got, again))            # no schedule in the result
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(25, 1000, 1030), (25, 1030, 1000)])
+def test_large_tiles_with_tiny_matrices_beside_them(shape):
+    """Enough work for the 256 x 256 tiles, which then also take matrices that fill a corner of one."""
+    big = momentum(shape, 11)
+    small = [momentum((3, 5, 7), 1), momentum((2, 64, 300), 2), momentum((65, 1), 3)]
+    got = ops.orthogonalize([big.cuda()] + [u.cuda() for u in small])
+    for i in (0, 24):
+        off(got[0][i], big[i])
+    for u, o in zip(small, got[1:]):
+        for a, b in zip(u.reshape(-1, *u.shape[-2:]), o.reshape(-1, *o.shape[-2:])):
+            off(b, a)
+    again = ops.orthogonalize(big.cuda())
+    assert torch.equal(again, got[0])
 
 
 @gpu
