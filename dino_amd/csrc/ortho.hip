@@ -260,15 +260,16 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
     static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
-    // parts of a stage: one panel of P and one of Q (SPLIT: its hi and lo), or (T = 128) two panels of both: fewer
-    // phases, which cost about 0.35 us each
-    static constexpr int KB = T == 128 && !SPLIT ? 2 : 1, PP = KB, QP = SPLIT ? 2 : KB;
+    // parts of a stage: KB panels of P and of Q (SPLIT: Q's hi, then its lo).  Two panels for T = 128: half the phases,
+    // whose fixed part (barrier, LDS latency: about 0.35 us) is otherwise longer than their products
+    static constexpr int KB = T == 128 ? 2 : 1, PP = KB, QP = SPLIT ? 2 * KB : KB;
     static constexpr int OPB = T * BK * 2, STAGE = (PP + QP) * OPB;
-    static constexpr int S = SPLIT ? 3 : T == 256 ? 4 : 2;          // 128 to 144 KB (T = 256), 64 to 72 KB (T = 128)
+    static constexpr int S = SPLIT ? 3 : T == 256 ? 4 : 2;
     static constexpr int ND = T / 128;                              // DMAs a wave and part
     static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
     static constexpr int IMG = SPLIT ? 0 : 16 * SUBM * 2;           // image of 16 columns of it (UPDATE has none)
-    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 144 to 160 KB / 72 to 80 KB: one / two workgroups a CU
+    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 160 KB (SPLIT: 144), T = 128 without SPLIT 80 KB
+    static constexpr int PER_CU = T == 128 && !SPLIT ? 2 : 1;       // workgroups a CU: LDS and registers allow so many
 };
 // The DMA is written in assembly: behind the builtin the compiler waits for ALL requests before every transposing LDS
 // read, which may alias what is being filled for all it knows.  It has no register result; the waits are landed()'s.
@@ -319,7 +320,7 @@ template <bool TOBF> DEVI unsigned pack2(float a, float b) {
 }
 
 template <int MODE, int T, bool SPLIT>
-__global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const GemmArgs ga) {
+__global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_kernel(const GemmArgs ga) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Cfg<T, SPLIT> C;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
@@ -378,9 +379,9 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
             for (int h = 0; h < QP; ++h)
 #pragma unroll
                 for (int u = 0; u < ND; ++u) {
-                    const int kp = SPLIT ? ik : ik * KB + h;   // panel along the contraction
+                    const int kp = ik * KB + h % KB;           // panel along the contraction
                     const int so = SYM ? (kp * imp + in0) * 64 : (min((in0 >> 5) + ((wave + 8 * u) >> 1), ilast) * imp + kp * 32) * 64;
-                    dma16(at + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h : 0], so);
+                    dma16(at + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h / KB : 0], so);
                 }
             ++issued;
             if (++ik == itotal) {
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(512, T == 128 ? 4 : 2) void ortho_gemm_kernel(const
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
                     acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        __builtin_bit_cast(f16x8, fq[h][ni]), __builtin_bit_cast(f16x8, fp[SPLIT ? 0 : h][mi]), acc[mi][ni], 0, 0, 0);
+                        __builtin_bit_cast(f16x8, fq[h][ni]), __builtin_bit_cast(f16x8, fp[h % KB][mi]), acc[mi][ni], 0, 0, 0);
     };
     auto phase = [&]() {
         asm volatile("" ::: "memory");
@@ -755,7 +756,7 @@ template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStre
         if (e != hipSuccess) return (int)e;
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    const int most = 256 * (T == 128 ? 2 : 1);        // what the CUs hold at once
+    const int most = 256 * Cfg<T, SPLIT>::PER_CU;     // what the CUs hold at once
     hipLaunchKernelGGL((ortho_gemm_kernel<MODE, T, SPLIT>), dim3(ga.ntiles < most ? ga.ntiles : most), dim3(512), smem, st, ga);
     return dino_launch_status();
 }
