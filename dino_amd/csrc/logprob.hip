@@ -204,11 +204,12 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
         for (int w = 0; w < NW; ++w) md = fmaxf(md, red[w]);
     }
     // (d - ref) / tau in units of log 2.  One fma an element: z = d sc - fl(ref sc), whose offset against the exact
-    // (d - ref) sc is the same dz for every element of the chunk and is taken out of the sums below.  Where ref sc
-    // itself is out of range (rows of the type's lowest value) the difference is formed first.
+    // (d - ref) sc is the same dz for every element of the chunk and is taken out of the sums below.  dz is half a step of
+    // ref sc: at most 1/4 below 2^22.  Rows further from zero (masked by -1e9 or the type's lowest value throughout) form
+    // the difference first.
     const float ref = md == NEG_INF ? 0.f : md, sc = a.inv_temp * LOG2E, off = ref * sc;
     float s = 0.f, t2 = 0.f;
-    if (fabsf(off) < 1e30f) {
+    if (fabsf(off) < 4194304.f) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll

@@ -148,6 +148,25 @@ def test_rows_masked_by_the_lowest_value(K):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [300, 20000])
+@pytest.mark.parametrize("base", [-1e9, 3e7, 1e20, -1e33])
+def test_rows_far_from_zero(base, K, dtype):
+    """A finite mask value in every column, or in all but one, and values that differ in their last bit only: what counts
+    is the distance to the row's largest.  The temperature is a power of two, so z of the definition is exact."""
+    low = torch.tensor(base, dtype=dtype)
+    high = torch.nextafter(low, torch.tensor(math.inf, dtype=dtype))
+    x = low.repeat(4, K)
+    x[1, K // 2:] = high
+    x[2, K // 3] = high
+    x[3, 5] = 0.25
+    tgt = torch.tensor([[0], [K - 1], [K // 3], [5]])
+    g = torch.Generator().manual_seed(K)
+    got = check(x, tgt, None, 2.0 ** -5, 3, g)
+    assert abs(got.entropy[0].item() - math.log(K)) < 1e-5
+
+
+@gpu
 @pytest.mark.parametrize("K", [200, 5000, 70000])
 def test_nan_and_infinity_stay_in_their_row(K):
     x, tgt, c, g = make(6, K, torch.float32, 1, 6)
