@@ -157,7 +157,7 @@ __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const 
 
 // X0 = U * SX 2^e / (|U| + eps) as hi + lo in panels, shorter side in front, padding cleared; 64 x 64 elements at a time,
 // through LDS where U is tall.  VEC: U's rows start at multiples of four elements.
-template <typename T, bool VEC> DEVI void prep_tiles(const Mat& q, const T* u, f16* xh, f16* xl, int t0, int t1, float scale, float (&tile)[64][66]) {
+template <typename T, bool VEC> DEVI void prep_tiles(const Mat& q, const T* u, f16* xh, f16* xl, int t0, int t1, float pre, float scale, float (&tile)[64][66]) {
     const int tn = (q.np + 63) / 64, c4 = (threadIdx.x & 15) * 4, r0 = threadIdx.x >> 4;
     for (int t = t0; t < t1; ++t) {
         const int m0 = (t / tn) * 64, n0 = (t % tn) * 64;
@@ -198,7 +198,7 @@ template <typename T, bool VEC> DEVI void prep_tiles(const Mat& q, const T* u, f
             f16x4 h, l;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float x = v[p][k] * scale;
+                const float x = v[p][k] * pre * scale;
                 h[k] = (f16)x;
                 l[k] = (f16)(x - (float)h[k]);
             }
@@ -216,20 +216,22 @@ __global__ __launch_bounds__(NTHR) void ortho_prep_kernel(const Ws ws, double ep
     double s = 0;
     for (int p = threadIdx.x; p < q.parts; p += NTHR) s += ws.parts[q.part0 + b * q.parts + p];
     const double norm = sqrt(block_sum_f64(s, red)), end = gain * (norm / (norm + eps));
-    const int e = end > 0.0 && end < 1.0 ? min(80, ilogb(1.0 / end)) : 0;
-    const float scale = (float)(ldexp((double)SX, e) / (norm + eps));
+    const int e = end > 0.0 && end < 1.0 ? min(120, ilogb(1.0 / end)) : 0;
+    // in two factors where one would leave fp32: a norm below 1e-35 with an eps as small
+    const double whole = ldexp((double)SX, e) / (norm + eps);
+    const float pre = whole > 0x1p100 ? 0x1p64f : 1.f, scale = (float)(whole / pre);
     if (part == 0 && threadIdx.x == 0) ws.exps[q.mat0 + b] = ldexpf(1.f, -e);
     const int nt = ((q.mp + 63) / 64) * ((q.np + 63) / 64), t0 = part * q.preps, t1 = min(nt, t0 + q.preps);
     const int64_t xo = q.xoff + (int64_t)b * q.mp * q.np;
     f16 *xh = ws.x[0][0] + xo, *xl = lo ? ws.x[0][1] + xo : nullptr;
     if (q.dtype == DINO_F32) {
         const float* u = (const float*)q.in + b * q.in_batch;
-        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 4)) & 15) == 0) prep_tiles<float, true>(q, u, xh, xl, t0, t1, scale, tile);
-        else prep_tiles<float, false>(q, u, xh, xl, t0, t1, scale, tile);
+        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 4)) & 15) == 0) prep_tiles<float, true>(q, u, xh, xl, t0, t1, pre, scale, tile);
+        else prep_tiles<float, false>(q, u, xh, xl, t0, t1, pre, scale, tile);
     } else {
         const bf16* u = (const bf16*)q.in + b * q.in_batch;
-        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 2)) & 7) == 0) prep_tiles<bf16, true>(q, u, xh, xl, t0, t1, scale, tile);
-        else prep_tiles<bf16, false>(q, u, xh, xl, t0, t1, scale, tile);
+        if ((((uintptr_t)u | (uint64_t)(q.in_ld * 2)) & 7) == 0) prep_tiles<bf16, true>(q, u, xh, xl, t0, t1, pre, scale, tile);
+        else prep_tiles<bf16, false>(q, u, xh, xl, t0, t1, pre, scale, tile);
     }
 }
 

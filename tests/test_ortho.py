@@ -128,6 +128,15 @@ def test_scale_of_the_update(scale):
 
 
 @gpu
+@pytest.mark.parametrize("scale,eps", [(1e-38, 0.0), (1e-41, 0.0), (1e-41, 1e-40), (1e-10, 1e20), (1e-3, 1e29)])
+def test_norms_at_the_end_of_the_range(scale, eps):
+    """1 / |U| is past fp32's range, or |U| / eps far below fp16's."""
+    u = momentum((60, 90), 4, "noise") * scale
+    off(ops.orthogonalize(u.cuda(), eps=eps), u, eps=eps)
+    off(ops.orthogonalize(u.t().contiguous().cuda(), eps=eps), u.t().contiguous(), eps=eps)
+
+
+@gpu
 def test_zeros_and_bad_numbers_stay_in_their_matrix():
     u = momentum((5, 70, 90), 3).cuda()
     clean = ops.orthogonalize(u)
