@@ -592,7 +592,12 @@ class OrthoPlan:
         _req(isinstance(eps, (int, float)) and 0.0 <= eps < 1e30, "eps", eps)
         outs = [None] * len(ups) if out is None else list(out)
         _req(len(outs) == len(ups), "out: one for each update")
+        given = [o.data_ptr() for o in outs if o is not None and o.numel()]
+        _req(len(set(given)) == len(given), "out: one tensor twice")
         self.out, self._updates, self._steps, self._eps = [], ups, steps, float(eps)
+        self._coeffs = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
+        # (no items: the checks of steps and coefficients only)
+        check(_lib.load().dino_ortho(None, 0, steps, self._coeffs, self._eps, None, 0, None), "dino_ortho")
         if not ups:
             return
         _dev(*ups, *outs)
@@ -612,7 +617,6 @@ class OrthoPlan:
                 q.out, q.out_batch, q.out_ld = self._place(o, r, c)
                 q.rows, q.cols, q.batch, q.dtype = r, c, shape[0] if len(shape) == 3 else 1, dt_code(u.dtype)
                 self.out.append(o)
-            self._coeffs = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
             need = ctypes.c_int64(0)
             check(_lib.load().dino_ortho_workspace(self._items, len(ups), ctypes.byref(need)), "dino_ortho_workspace")
             self._need = need.value
@@ -639,7 +643,8 @@ def orthogonalize(updates, *, steps=5, coeffs=NS_COEFFS, eps=1e-7, out=None):
     """Orthogonalised updates by Newton-Schulz products (include/dino_hip.h: dino_ortho), all matrices in one sequence of
     launches.  updates: a tensor or a list of tensors, each [rows, cols] or [batch, rows, cols] in fp32 / bf16, columns
     side by side, rows with any stride.  coeffs: (a, b, c), or one such triple per step.  Returns bf16 tensors of the same
-    shapes (a tensor for a tensor, a list for a list); out: the caller's own, in the same form."""
+    shapes (a tensor for a tensor, a list for a list); out: the caller's own, in the same form (they may overlap the updates,
+    not each other)."""
     if isinstance(updates, torch.Tensor):
         return OrthoPlan([updates], None if out is None else [out], steps=steps, coeffs=coeffs, eps=eps).run()[0]
     return OrthoPlan(updates, out, steps=steps, coeffs=coeffs, eps=eps).run()

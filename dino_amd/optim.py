@@ -194,6 +194,7 @@ class FusedMuon(FusedAdamW):
             raise ValueError(f"FusedMuon: momentum {momentum} is not in [0, 1)")
         if scale not in ("rms", "spectral"):
             raise ValueError(f"FusedMuon: scale is \"rms\" or \"spectral\", got {scale!r}")
+        ops.OrthoPlan([], steps=ns_steps, coeffs=ns_coeffs, eps=ns_eps)          # refuses what no step could use
         super().__init__(params, student, teacher, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         self.momentum, self.nesterov = float(momentum), bool(nesterov)
         self.ns_steps, self.ns_coeffs, self.ns_eps = ns_steps, ns_coeffs, float(ns_eps)

@@ -313,9 +313,9 @@ int dino_adamw_ema(float* param, const float* grad, float* exp_avg, float* exp_a
 /* Orthogonalised updates (Muon; no counterpart in the reference, whose optimiser is AdamW): for each of `count` items, a
  * stack of `batch` matrices U [rows, cols] (dtype DINO_F32 / DINO_BF16, element strides in_batch / in_ld, columns side by
  * side),  X = U / (|U|_F + eps), then per step  X <- a X + (b A + c A A) X  with A = X X^T (the shorter side of U in
- * front),  (a, b, c) = coeffs[3 * step ..] (host).  out: bf16 [batch, rows, cols] (out_batch, out_ld).  out may be `in` of a
- * bf16 item of the same strides.  Products take fp16 operands (pairs of them while a rounding error would still grow
- * more than 16 times) and fp32 sums.  coeffs must keep the singular values below 12 (checked on the host:
+ * front),  (a, b, c) = coeffs[3 * step ..] (host).  out: bf16 [batch, rows, cols] (out_batch, out_ld).  Outputs may
+ * overlap inputs (all are read before the first result is written), not each other.  Products take fp16 operands (pairs of them while a rounding error would still grow
+ * more than 8 times) and fp32 sums.  coeffs must keep the singular values below 12 (checked on the host:
  * DINO_ERR_BADARG).  rows, cols <= 32768 and rows * cols < 2^30, else DINO_ERR_TOO_LARGE.  NaN or infinity stays in its matrix; a
  * matrix of zeros gives zeros (eps > 0).  workspace: dino_ortho_workspace bytes, 256-byte aligned, used by this call alone. */
 #define DINO_ORTHO_MAX_STEPS 16

@@ -162,6 +162,29 @@ def test_watch_matches_plain_code(dtype):
 
 
 @gpu
+def test_no_hidden_matrix_is_adamw():
+    """select can take none: then every parameter is AdamW's."""
+    from dino_amd.optim import FusedAdamW
+    from dino_amd.utils import get_params_groups
+    runs = []
+    for muon in (True, False):
+        student, teacher, loss_fn, opt, crops = _setup(torch.float32, select=lambda k, p: False)
+        if not muon:
+            opt = FusedAdamW(get_params_groups(student), student, teacher)
+        _backward(student, teacher, loss_fn, opt, crops, 0)
+        g = {k: p.grad.clone() for k, p in student.named_parameters() if p.grad is not None}
+        runs.append((g, {k: p.detach().clone() for k, p in student.named_parameters()}, opt, student))
+    for g, _, opt, student in runs:                       # the same gradients for both (they are added with float atomics)
+        for k, p in student.named_parameters():
+            if p.grad is not None:
+                p.grad.copy_(runs[0][0][k])
+        opt.step(ema_momentum=0.9)
+    a, b = (dict(r[3].named_parameters()) for r in runs)
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_prototype_log_probs_and_its_gradient(dtype):
     from dino_amd.components import prototype_log_probs
@@ -236,12 +259,24 @@ def test_training_with_both_together():
 
 
 def test_refusals_on_the_cpu():
+    from dino_amd._lib import DinoHipError
     from dino_amd.components import prototype_log_probs
+    from dino_amd.components.loss import DINOLoss
     from dino_amd.optim import FusedMuon, is_hidden_matrix
     p = torch.nn.Parameter(torch.zeros(4, 4))
     for kw in (dict(momentum=1.0), dict(momentum=-0.1), dict(scale="other")):
         with pytest.raises(ValueError):
             FusedMuon([p], torch.nn.Linear(2, 2), **kw)
+    for kw in (dict(ns_steps=0), dict(ns_coeffs=(1.0, 2.0)), dict(ns_coeffs=(20.0, 0.0, 0.0)), dict(ns_eps=-1.0)):
+        with pytest.raises(DinoHipError):
+            FusedMuon([p], torch.nn.Linear(2, 2), **kw)
+    loss_fn = DINOLoss(10, 4, 0.04, 0.04, 0, 3)
+    with pytest.raises(ValueError):
+        loss_fn.watch(torch.zeros(7, 10), torch.zeros(4, 10), 0)            # 4 crops of 2 images are 8 rows
+    lazy = torch.zeros(8, 10)
+    lazy._dino_lazy = object()
+    with pytest.raises(ValueError):
+        loss_fn.watch(lazy, torch.zeros(4, 10), 0)
     with pytest.raises(ValueError):
         prototype_log_probs(torch.zeros(2, 5), center=torch.zeros(5, requires_grad=True))
     assert is_hidden_matrix("backbone.blocks.3.attn.qkv.weight", p) and is_hidden_matrix("head.mlp.2.weight", p)

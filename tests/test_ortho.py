@@ -128,6 +128,27 @@ def test_scale_of_the_update(scale):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(32704, 32768), (32768, 16400)])
+def test_largest_matrices(shape):
+    """Offsets up to the last byte that a matrix may have (2^31).  Zeros but for blocks in the corners and between: rows and
+    columns of zeros stay zeros, and every block takes the recurrence from its part of the whole norm."""
+    r, c = shape
+    at = [(0, 0), (r // 2 + 3, c // 3 + 1), (r - 90, c - 120)]
+    u = torch.zeros(shape, device="cuda")
+    blocks = [momentum((90, 120), 60 + i, "noise") for i in range(3)]
+    for (y, x), b in zip(at, blocks):
+        u[y:y + 90, x:x + 120] = b.cuda()
+    got = ops.orthogonalize(u)
+    whole = math.sqrt(sum(b.double().square().sum().item() for b in blocks))
+    inside = 0
+    for (y, x), b in zip(at, blocks):
+        o = got[y:y + 90, x:x + 120]
+        inside += torch.count_nonzero(o).item()
+        off(o, b, eps=whole - torch.linalg.vector_norm(b.double()).item() + 1e-7)
+    assert torch.count_nonzero(got).item() == inside > 0
+
+
+@gpu
 @pytest.mark.parametrize("scale,eps", [(1e-38, 0.0), (1e-41, 0.0), (1e-41, 1e-40), (1e-10, 1e20), (1e-3, 1e29)])
 def test_norms_at_the_end_of_the_range(scale, eps):
     """1 / |U| is past fp32's range, or |U| / eps far below fp16's."""
@@ -227,6 +248,9 @@ def test_refusals_on_the_cpu(monkeypatch):
         ops.orthogonalize(torch.zeros(4, 6, dtype=torch.float16))
     with pytest.raises(DinoHipError):
         ops.orthogonalize([u, u], out=[torch.zeros(4, 6, dtype=torch.bfloat16)])
+    twice = torch.zeros(4, 6, dtype=torch.bfloat16)
+    with pytest.raises(DinoHipError):
+        ops.orthogonalize([u, u], out=[twice, twice])
     assert ops.orthogonalize([]) == []
 
 
