@@ -480,7 +480,7 @@ Plan plan_of(int64_t rows, int K) {
     const int most = K <= 8192 * MAX_CHUNKS ? 4 : 8;
     while (p.nv < most && p.nt * 8 * p.nv < K) p.nv *= 2;
     // few rows: shorter chunks, so that a row is read by many CUs
-    if (K > 4096)
+    if (K > 8192)
         while (p.nv > 1) {
             const int64_t next = (K + p.nt * 4 * p.nv - 1) / (p.nt * 4 * p.nv);
             if (next > MAX_CHUNKS || rows * next > 1024) break;

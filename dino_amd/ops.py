@@ -465,25 +465,35 @@ LOGPROB_MAX_TOPK, LOGPROB_MAX_TARGETS = 64, 4096
 
 
 def _logprob_operands(logits, targets, center, temp):
-    """(rows, K, T, row stride, inverse temperature) of checked operands."""
+    """(rows, K, T, row stride, inverse temperature) of checked operands.  (A small call is the host's time: what a refusal
+    says is put together only when there is one.)"""
     _dev(logits, targets, center)
-    _req(logits.dim() == 2, "logits: [R, K]", logits.shape)
-    R, K = logits.shape
+    shape = logits.shape
+    if len(shape) != 2:
+        _req(False, "logits: [R, K]", shape)
+    R, K = shape
     ld, one = logits.stride()
-    _req(K > 0 and (one == 1 or K == 1), "logits: columns side by side", logits.shape, logits.stride())
-    _req(R <= 1 or ld >= K, "logits: rows overlap", logits.stride())
-    T = 0
+    if K == 0 or (one != 1 and K != 1):
+        _req(False, "logits: columns side by side", shape, (ld, one))
+    if R > 1 and ld < K:
+        _req(False, "logits: rows overlap", (ld, one))
+    dev, T = logits.device, 0
     if targets is not None:
-        _req(targets.dtype is torch.int64 and targets.dim() == 2 and targets.shape[0] == R and targets.is_contiguous(),
-             "targets: contiguous int64 [R, T]", targets.dtype, targets.shape)
-        T = targets.shape[1]
-        _req(T <= LOGPROB_MAX_TARGETS, f"at most {LOGPROB_MAX_TARGETS} targets a row", T)
-        _req(targets.device == logits.device, "operands on different devices")
+        ts = targets.shape
+        if targets.dtype is not torch.int64 or len(ts) != 2 or ts[0] != R or not targets.is_contiguous():
+            _req(False, "targets: contiguous int64 [R, T]", targets.dtype, ts)
+        T = ts[1]
+        if T > LOGPROB_MAX_TARGETS:
+            _req(False, f"at most {LOGPROB_MAX_TARGETS} targets a row", T)
+        if targets.device != dev:
+            _req(False, "operands on different devices")
     if center is not None:
-        _req(center.dtype is torch.float32 and center.is_contiguous() and center.numel() == K,
-             "center: contiguous float32, one value a column", center.dtype, center.shape)
-        _req(center.device == logits.device, "operands on different devices")
-    _req(isinstance(temp, (int, float)) and 1e-37 < temp < 1e37, "temperature: positive and finite", temp)
+        if center.dtype is not torch.float32 or not center.is_contiguous() or center.numel() != K:
+            _req(False, "center: contiguous float32, one value a column", center.dtype, center.shape)
+        if center.device != dev:
+            _req(False, "operands on different devices")
+    if not (isinstance(temp, (int, float)) and 1e-37 < temp < 1e37):
+        _req(False, "temperature: positive and finite", temp)
     return R, K, T, max(ld, K), 1.0 / temp
 
 
@@ -499,8 +509,8 @@ def logprob_fwd(logits, targets=None, *, center=None, temp=1.0, topk=0) -> LogPr
     (include/dino_hip.h: dino_logprob_fwd).  logits [R, K] bf16 / fp32 with any row stride; targets int64 [R, T]
     (-1: none) or None; center fp32 [K] or None."""
     R, K, T, ld, inv = _logprob_operands(logits, targets, center, temp)
-    _req(isinstance(topk, int) and 0 <= topk <= min(K, LOGPROB_MAX_TOPK),
-         f"topk between 0 and min(K, {LOGPROB_MAX_TOPK})", topk)
+    if not (isinstance(topk, int) and 0 <= topk <= min(K, LOGPROB_MAX_TOPK)):
+        _req(False, f"topk between 0 and min(K, {LOGPROB_MAX_TOPK})", topk)
     dt, dev, f32 = dt_code(logits.dtype), logits.device, torch.float32
     need = _logprob_workspace(R, K, topk)
     with _on(dev):
@@ -527,24 +537,29 @@ def logprob_bwd(logits, fwd: LogProbs, *, targets=None, center=None, temp=1.0, d
     ent, stats, tix = fwd.entropy, fwd.stats, fwd.top_index
     k = 0 if tix is None else tix.shape[1]
     dev = logits.device
-    _dev(ent, stats, tix, dlog_prob, dentropy, dtop_log_prob, dlogits)
-    _f32(ent, stats, dlog_prob, dentropy, dtop_log_prob)
-    _req(stats.shape == (R, 2) and ent.shape == (R,), "forward results of other logits")
-    _req(dlog_prob is None or (targets is not None and dlog_prob.shape == (R, T)), "dlog_prob: [R, T], with its targets")
-    _req(dentropy is None or dentropy.shape == (R,), "dentropy: [R]")
-    _req(dtop_log_prob is None or (k > 0 and dtop_log_prob.shape == (R, k)), "dtop_log_prob: [R, topk]")
-    _req(tix is None or (tix.dtype is torch.int64 and tix.is_contiguous() and tix.shape[0] == R), "top_index")
-    for t in (ent, stats, tix, dlog_prob, dentropy, dtop_log_prob, dlogits):
-        _req(t is None or t.device == dev, "operands on different devices")
+    for t, shape, what in ((ent, (R,), "entropy"), (stats, (R, 2), "stats"), (dlog_prob, (R, T), "dlog_prob"),
+                           (dentropy, (R,), "dentropy"), (dtop_log_prob, (R, k), "dtop_log_prob")):
+        if t is not None and not (t.dtype is torch.float32 and t.shape == shape and t.device == dev and t.is_contiguous()):
+            _req(False, f"{what}: contiguous float32, here {shape} on the logits' device", t.dtype, t.shape)
+    if dlog_prob is not None and targets is None:
+        _req(False, "dlog_prob needs its targets")
+    if dtop_log_prob is not None and tix is None:
+        _req(False, "dtop_log_prob needs the forward's top_index")
+    if tix is not None and not (tix.dtype is torch.int64 and tix.is_contiguous() and tix.shape[0] == R and tix.device == dev):
+        _req(False, "top_index of other logits")
+    ldd = K
+    if dlogits is not None:
+        if not (dlogits.shape == (R, K) and dlogits.dtype is logits.dtype and dlogits.device == dev
+                and (dlogits.stride(1) == 1 or K == 1) and (R <= 1 or dlogits.stride(0) >= K)):
+            _req(False, "dlogits: [R, K] of the logits' type, on their device")
+        ldd = max(dlogits.stride(0), K)
     with _on(dev):
         if dlogits is None:
-            dlogits = torch.empty((R, K), dtype=logits.dtype, device=dev)
-        _req(dlogits.shape == (R, K) and dlogits.dtype == logits.dtype and (dlogits.stride(1) == 1 or K == 1)
-             and (R <= 1 or dlogits.stride(0) >= K), "dlogits: [R, K] of the logits' type")
+            dlogits = logits.new_empty((R, K))
         check(_lib.load().dino_logprob_bwd(
             dt_code(logits.dtype), logits.data_ptr(), ld, R, K, _ptr(center), inv, stats.data_ptr(), ent.data_ptr(),
             _ptr(targets), T, _ptr(dlog_prob), _ptr(dentropy), _ptr(tix), k, _ptr(dtop_log_prob), dlogits.data_ptr(),
-            max(dlogits.stride(0), K), _stream()), "dino_logprob_bwd")
+            ldd, _stream()), "dino_logprob_bwd")
     return dlogits
 
 

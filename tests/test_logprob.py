@@ -355,6 +355,26 @@ def test_refusals_on_the_cpu(monkeypatch):
             ops.logprob_fwd(odd)
 
 
+def test_backward_refusals_on_the_cpu(monkeypatch):
+    monkeypatch.setattr(ops, "_dev", lambda *a: None)
+    i64, bf = torch.int64, torch.bfloat16
+    x, tgt = torch.zeros(2, 9), torch.zeros(2, 1, dtype=i64)
+    r = ops.LogProbs(torch.zeros(2, 1), torch.zeros(2), torch.zeros(2, 2), torch.zeros(2, 3), torch.zeros(2, 3, dtype=i64))
+    bad = [
+        dict(dlog_prob=torch.zeros(2, 1)), dict(targets=tgt, dlog_prob=torch.zeros(2, 2)),
+        dict(targets=tgt, dlog_prob=torch.zeros(2, 1, dtype=bf)), dict(dentropy=torch.zeros(3)),
+        dict(dentropy=torch.zeros(2, dtype=torch.float64)), dict(dtop_log_prob=torch.zeros(2, 2)),
+        dict(dtop_log_prob=torch.zeros(3, 2).t()), dict(dlogits=torch.zeros(2, 9, dtype=bf)), dict(dlogits=torch.zeros(2, 8)),
+        dict(dlogits=torch.zeros(9, 2).t()), dict(dlogits=torch.zeros(1, 9).expand(2, 9)), dict(temp=0.0),
+        dict(fwd=r._replace(stats=torch.zeros(3, 2))), dict(fwd=r._replace(entropy=torch.zeros(2, 1))),
+        dict(fwd=r._replace(top_index=torch.zeros(2, 3, dtype=torch.int32))),
+        dict(fwd=r._replace(top_index=None, top_log_prob=None), dtop_log_prob=torch.zeros(2, 3)),
+    ]
+    for kw in bad:
+        with pytest.raises(DinoHipError):
+            ops.logprob_bwd(x, kw.pop("fwd", r), **kw)
+
+
 def test_entry_points_refuse_bad_arguments():
     import ctypes
 
