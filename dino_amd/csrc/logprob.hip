@@ -468,8 +468,11 @@ __global__ __launch_bounds__(BNT) void logprob_bwd_kernel(const BwdArgs a) {
     }
 }
 
-// Columns per workgroup: 32 a thread (64 where 64 chunks of 8192 would not reach the end).  Rows of up to
-// 8192 columns are one workgroup's (one wave's up to 2048); longer ones are cut into chunks that a second kernel joins.
+// Columns per workgroup.  A row of up to 16384 is one workgroup's, up to 64 columns a thread (one wave's up to 2048): no
+// second launch.  Two chunks and a join against it, us on MI355X: 333 rows of 8191 (fp32, topk 5) 10.4 / 6.8; of 16384, bf16
+// with topk 5: 1 row 8.5 / 6.9, 512 13.4 / 9.4, 2560 28.2 / 23.8, 12608 125 / 113.
+// Longer rows are cut into chunks of 8192, 32 columns a thread (512 rows of 65536 bf16, centred, topk 8: 26 us; chunks of
+// 16384: 27), joined by a second kernel; of 16384 where 64 chunks would not reach the end.
 struct Plan {
     int nt, nv, chunk, S;
 };
@@ -477,10 +480,10 @@ Plan plan_of(int64_t rows, int K) {
     Plan p;
     p.nt = K <= 2048 ? 64 : K <= 4096 ? 128 : 256;
     p.nv = 1;
-    const int most = K <= 8192 * MAX_CHUNKS ? 4 : 8;
+    const int most = K > 16384 && K <= 8192 * MAX_CHUNKS ? 4 : 8;
     while (p.nv < most && p.nt * 8 * p.nv < K) p.nv *= 2;
-    // few rows: shorter chunks, so that a row is read by many CUs
-    if (K > 8192)
+    // few rows: shorter chunks, so that a row is read by many CUs (1 row of 65536: 32 chunks of 2048)
+    if (K > 16384)
         while (p.nv > 1) {
             const int64_t next = (K + p.nt * 4 * p.nv - 1) / (p.nt * 4 * p.nv);
             if (next > MAX_CHUNKS || rows * next > 1024) break;

@@ -266,7 +266,7 @@ int dino_proto_loss_chunk(int dtype, int phase, void* s_chunk, int64_t lds, cons
  *   top_index / top_log_prob [rows, topk]  the largest d, equal ones by their index (topk <= 64, 0: none)
  * logits: dtype [rows, K], row stride ld (any; rows need no alignment beyond the element's).  -inf logits have
  * probability 0; a row of nothing else gives log_prob -inf, entropy 0 and gradient 0.  NaN or +inf: NaN for the row.
- * K <= 1048576 (else DINO_ERR_TOO_LARGE).  workspace: dino_logprob_workspace bytes (0 for K <= 4096), of this call alone.
+ * K <= 1048576 (else DINO_ERR_TOO_LARGE).  workspace: dino_logprob_workspace bytes (0 for K <= 16384), of this call alone.
  * Backward: dlogits [rows, K] (row stride ldd, may be logits itself) = gradient of
  *   sum dlog_prob * log_prob + sum dentropy * entropy + sum dtop_log_prob * top_log_prob   (each nullable),
  * rounded to dtype once.  center is a constant.  T <= 4096.

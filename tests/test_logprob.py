@@ -114,7 +114,8 @@ def check(x, tgt, c, temp, topk, g, grads=True):
 
 # every variant of the kernel (one wave, 1 to 8 vectors; one chunk; many chunks), ends inside a vector
 SIZES = [(1, 1), (3, 2), (5, 9), (4, 65), (7, 512), (2, 777), (3, 1025), (2, 2047), (3, 4096), (2, 4097), (5, 8191),
-         (1, 16385), (2, 65536), (9, 65537), (1, 100003), (2, 524289), (1, 1048576), (70001, 33)]
+         (1, 16385), (2, 65536), (9, 65537), (1, 100003), (3, 9000), (2, 16384),
+         (2, 524289), (1, 1048576), (70001, 33)]
 
 
 @gpu
