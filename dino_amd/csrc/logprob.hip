@@ -135,6 +135,10 @@ DEVI void put_top(const FwdArgs& a, int64_t row, int j, u64 key, float md, float
 
 // One workgroup of NT threads takes one chunk (at most NT * 8 * NV columns) of one row, held in registers: read
 // once, then the maximum, the sums and the best k come from registers.
+// Bound: memory, with about 12 vector instructions and an exp2 an element close behind (50 us of the 85 below).  MI355X:
+// 2560 rows of 65536 bf16 (336 MB) 80 .. 86 us = 4.0 TB/s; 512 of them with a centre (it stays in L2) and 8 best (67 MB)
+// 24 us = 2.8 TB/s; 12608 of 4096 with 2 best (103 MB) 25 us = 4.1 TB/s; 333 fp32 rows of 8191, a third of them -inf, 9.7 us.
+// Splitting a row over workgroups of 256 threads leaves 32 values a thread in registers, five waves a SIMD or more.
 template <typename T, int NT, int NV, bool CEN>
 __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
     constexpr int NW = NT / 64;
@@ -289,13 +293,27 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
                 if (rank < k) best[rank] = key;
             }
             __syncthreads();
-        } else {      // many equal or masked values, or a NaN: k rounds of the next best key, columns read again
+        } else if (md == NEG_INF && !nan) {          // nothing but -inf: the first ones
+            for (int q = tid; q < k; q += NT) best[q] = c0 + q < c1 ? make_key(NEG_INF, c0 + q) : 0;
+            __syncthreads();
+        } else {
+            // many equal or masked values, or a NaN: k rounds of the next best key.  The columns are read again, eight loads at
+            // a time: d kept alive to here costs registers in every row (12608 rows of 4096: 25.3 us without, 28.7 with)
             u64 last = ~0ull;
             for (int q = 0; q < k; ++q) {
                 u64 mine = 0;
-                for (int at = c0 + tid; at < c1; at += NT) {
-                    const u64 key = make_key(to_f32<T>(x[at]) - (a.center ? a.center[at] : 0.f), at);
-                    if (key < last && key > mine) mine = key;
+                for (int b = c0 + tid; b < c1; b += 8 * NT) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int at = min(b + i * NT, c1 - 1);
+                        v[i] = to_f32<T>(x[at]) - (CEN ? a.center[at] : 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const u64 key = make_key(v[i], min(b + i * NT, c1 - 1));
+                        if (key < last && key > mine) mine = key;
+                    }
                 }
                 mine = wave_max_u64(mine);
                 if (NW > 1) {
@@ -321,7 +339,8 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
     }
 }
 
-// joins the chunks of a row: one wave per row, lane = chunk (at most 64)
+// joins the chunks of a row: one wave per row, lane = chunk (at most 64).  4 .. 6 us: latency of the launch and of topk
+// rounds over the chunks' sorted keys.
 template <typename T> __global__ __launch_bounds__(64) void logprob_join_kernel(const FwdArgs a) {
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
@@ -368,6 +387,7 @@ constexpr int BNT = 256, BNV = 4, BCHUNK = BNT * 8 * BNV;
 
 // dx_k = (sum_j g_j [k = idx_j] - p_k (sum_j g_j + gH (log p_k + H))) / tau; the (index, gradient) pairs of the row that
 // fall into the chunk are compacted in their order, so a repeated index adds up the same way every time.
+// Bound: memory.  One read, one write: 2560 rows of 65536 bf16 (671 MB) 113 us = 5.9 TB/s; 12608 of 4096 (207 MB) 38 us.
 template <typename T>
 __global__ __launch_bounds__(BNT) void logprob_bwd_kernel(const BwdArgs a) {
     extern __shared__ __attribute__((aligned(8))) char smem[];
