@@ -417,6 +417,10 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         const int row = 8 * g + (i >> 2), col = wn * C::SUBN + ni * 16, ch = (col & 31) / 8 + ((i & 3) >> 1);
         offT[ni] = PP * C::OPB + (col >> 5) * 2048 + row * 64 + ((ch ^ tkey(row)) << 4) + (i & 1) * 8;
     }
+    // LATER: a slot is refilled a phase later than its last read (one phase less ahead), and no wait for that read stands in
+    // front of the barrier: the products wait for their own operands as they come.  X' of pairs of ViT-L's matrices 1205 ->
+    // 1056 us, A 398 -> 385.  With two stages there is no phase to spare.
+    constexpr bool LATER = S > 2;
     u32x4 fp[PP][MI], fq[QP][NI];
     int slot = 0;
     auto read = [&]() {
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         for (int h = 0; h < PP; ++h)
 #pragma unroll
             for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(st + h * C::OPB + offP + x * 1024);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (!LATER) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     auto multiply = [&]() {
 #pragma unroll
@@ -608,25 +612,28 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
     };
 
     // ---- the stream of stages.  Early waves read stage s in phase 2s and multiply in 2s + 1, late ones a phase later; a
-    // tile that ended with s is finished by both in phase 2s + 2, where stage s + S is requested into the slot of s.
+    // tile that ended with s is finished by both in phase 2s + 2.  Stage s + S is requested into the slot of s in phase
+    // 2s + 2, LATER in 2s + 3: early waves' reads are waited for by their products in 2s + 1, late ones' in 2s + 2 (or at
+    // the end of 2s + 1).
     for (int s = 0; s < S - 1; ++s) issue();
     Tile cur = load_tile(tiles + b0), nxt = load_tile(tiles + b0 + (nmine > 1 ? G : 0));
     int total = (MODE == GRAM ? cur.np : cur.mp) / (BK * KB), j = 0, k = 0;
     float e1 = load_const(ws.exps + cur.all);
     landed(0);
     phase();
-    issue();
+    if (!LATER) issue();
     if (late) phase();
     for (int s = 0;; ++s) {
+        if (late && LATER) issue();
         read();
         if (late) landed(s + 1);
         phase();
-        if (late) issue();
+        if (late != LATER) issue();
         multiply();
         if (!late) {
             landed(s + 1);
             phase();
-            issue();
+            if (!LATER) issue();
         }
         if (++k == total) {
             finish(cur, e1);
