@@ -331,7 +331,8 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, i = lane & 15, g = lane >> 4;
-    const bool late = wave >= 4;
+    int late = wave >> 2;
+    asm volatile("" : "+s"(late));             // (an integer to the compiler, compared by scalar instructions)
     const Ws& ws = ga.ws;
     const Tile* tiles = SYM ? ws.sym : ws.rect;
     // workgroup -> tiles b, b + G, ...: in every round an XCD has neighbouring tiles
@@ -352,15 +353,19 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         voQ[u] = SYM ? voP[u] : t * 64 + (((lane & 3) ^ tkey(t)) << 4);
     }
     u32x4 rsP, rsQ[SPLIT ? 2 : 1];
-    const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem;
-    int ji = 0, ik = 0, itotal = 0, imp = 0, im0 = 0, in0 = 0, ilast = 0, islot = 0, issued = 0;
+    const unsigned lds0 = (unsigned)(uintptr_t)(lptr_t)smem + wave * 1024;
+    // the next stage to request: its tile's index, stages left in the tile, LDS address, offsets in P and Q, their steps
+    int ji = 0, left = 0, soP = 0, soQ[ND], panel = 0, stepQ = 0;
+    unsigned iat = lds0;
     Tile tn = load_tile(tiles + b0);                       // the tile after the one being requested
     auto open = [&]() {                        // start requesting tile tn
-        imp = tn.mp;
-        im0 = tn.m0;
-        in0 = tn.n0;
-        ilast = (tn.np >> 5) - 1;
-        itotal = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
+        panel = tn.mp * 64;
+        stepQ = KB * (SYM ? panel : 2048);
+        soP = tn.m0 * 64;
+#pragma unroll
+        for (int u = 0; u < ND; ++u)
+            soQ[u] = SYM ? tn.n0 * 64 : min((tn.n0 >> 5) + ((wave + 8 * u) >> 1), (tn.np >> 5) - 1) * panel;
+        left = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
         rsP = rsrc(MODE == GRAM ? ws.x[ga.src][0] + tn.xo : MODE == POLY ? ws.a + tn.ao : ws.b + tn.ao,
                    tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
 #pragma unroll
@@ -369,37 +374,40 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         if (ji + 1 < nmine) tn = load_tile(tiles + b0 + (ji + 1) * G);
     };
     open();
-    auto issue = [&]() {
-        if (ji < nmine) {
-            const unsigned at = lds0 + islot * C::STAGE + wave * 1024;
+    constexpr int NREQ = (PP + QP) * ND;                   // requests of a wave and stage
+    auto request = [&](int n) {
+        const int u = n % ND;
+        if (n < PP * ND) {
+            const int h = n / ND;
+            dma16(iat + h * C::OPB + u * 8192, voP[u], rsP, soP + h * panel);
+        } else {
+            const int h = n / ND - PP;                     // (h % KB: panel along the contraction)
+            dma16(iat + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h / KB : 0], soQ[u] + (h % KB) * (SYM ? panel : 2048));
+        }
+    };
+    // (Behind the last tile the requests go on, to the last matrix's first rows: a stage is always NREQ of them.)
+    auto requested = [&]() {
+        soP += KB * panel;
 #pragma unroll
-            for (int h = 0; h < PP; ++h)
+        for (int u = 0; u < ND; ++u) soQ[u] += stepQ;
+        iat += C::STAGE;
+        if (iat == lds0 + S * C::STAGE) iat = lds0;
+        if (--left == 0) {
+            if (++ji < nmine) open();
+            else {
+                soP = panel = stepQ = 0;
 #pragma unroll
-                for (int u = 0; u < ND; ++u)
-                    dma16(at + h * C::OPB + u * 8192, voP[u], rsP, ((ik * KB + h) * imp + im0) * 64);
-#pragma unroll
-            for (int h = 0; h < QP; ++h)
-#pragma unroll
-                for (int u = 0; u < ND; ++u) {
-                    const int kp = ik * KB + h % KB;           // panel along the contraction
-                    const int so = SYM ? (kp * imp + in0) * 64 : (min((in0 >> 5) + ((wave + 8 * u) >> 1), ilast) * imp + kp * 32) * 64;
-                    dma16(at + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h / KB : 0], so);
-                }
-            ++issued;
-            if (++ik == itotal) {
-                ik = 0;
-                if (++ji < nmine) open();
+                for (int u = 0; u < ND; ++u) soQ[u] = 0;
             }
         }
-        islot = islot + 1 == S ? 0 : islot + 1;
     };
-    auto landed = [&](int s) {       // my DMAs of stage s are done
-        const int younger = issued - 1 - s;
-        // (at most S - 1 stages are younger; where the stream ends the count falls below S - 2: then all but one)
-        if (younger >= S - 2) wait_vmcnt<(PP + QP) * ND * (S - 2)>();
-        else if (S == 4 && younger == 1) wait_vmcnt<(PP + QP) * ND>();
-        else wait_vmcnt<0>();
+    auto issue = [&]() {
+#pragma unroll
+        for (int n = 0; n < NREQ; ++n) request(n);
+        requested();
     };
+    // my DMAs of the next stage to read are done: at most S - 2 stages are younger
+    auto landed = [&]() { wait_vmcnt<NREQ * (S - 2)>(); };
 
     f32x4 acc[MI][NI];
     auto clear = [&]() {
@@ -444,15 +452,20 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
             for (int x = 0; x < MI; ++x) fp[h][x] = *(const u32x4*)(st + h * C::OPB + offP + x * 1024);
         if (!LATER) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    auto multiply = [&]() {
+    // with the requests of a stage between the products, whose time they then do not take
+    auto multiply = [&](bool req) {
 #pragma unroll
         for (int h = QP - 1; h >= 0; --h)
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi)
+            for (int mi = 0; mi < MI; ++mi) {
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni)
                     acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                         __builtin_bit_cast(f16x8, fq[h][ni]), __builtin_bit_cast(f16x8, fp[h % KB][mi]), acc[mi][ni], 0, 0, 0);
+                const int n = (QP - 1 - h) * MI + mi;
+                if (n < NREQ && req) request(n);
+                if (n == NREQ && req) requested();
+            }
     };
     auto phase = [&]() {
         asm volatile("" ::: "memory");
@@ -619,19 +632,20 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
     Tile cur = load_tile(tiles + b0), nxt = load_tile(tiles + b0 + (nmine > 1 ? G : 0));
     int total = (MODE == GRAM ? cur.np : cur.mp) / (BK * KB), j = 0, k = 0;
     float e1 = load_const(ws.exps + cur.all);
-    landed(0);
+    landed();
     phase();
     if (!LATER) issue();
     if (late) phase();
-    for (int s = 0;; ++s) {
-        if (late && LATER) issue();
+    for (;;) {
         read();
-        if (late) landed(s + 1);
+        if (late) {
+            if (LATER) issue();
+            landed();
+        }
         phase();
-        if (late != LATER) issue();
-        multiply();
+        multiply(LATER ? !late : late);
         if (!late) {
-            landed(s + 1);
+            landed();
             phase();
             if (!LATER) issue();
         }
@@ -646,6 +660,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         }
         if (late) phase();
     }
+    wait_vmcnt<0>();                            // no request outlives the workgroup's LDS
 #endif
 }
 
