@@ -253,12 +253,15 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 // Operands go global -> LDS by DMA in a ring of S stages of 32 along the contraction, one stream of stages over all tiles of
 // the workgroup: the next tile's first stages are on their way while this one's results leave.  With SPLIT (an UPDATE) a
 // stage holds the hi and the lo part of X and feeds two products.
-// What bounds it, for X' of ViT-L's 144 matrices (0.62 TFLOP; 0.9 GB to read, 0.6 GB to write): 610 us = 1010 TFLOP/s (a large
-// library product reaches 1306 here).  Alone, the requests take 329 us, the products 282, reading fragments and products
-// 390, all but writing the results 442: no single one bounds it, the phases do not overlap them fully.
+// What bounds it, for X' of ViT-L's 144 matrices (0.62 TFLOP; 0.9 GB to read, 0.6 GB to write): 590 us = 1050 TFLOP/s (a large
+// library product reaches 1306 here); of pairs (1.24 TFLOP) 1030 us = 1200.  The matrix pipes are busy in 57 % of the cycles (pairs:
+// 66 %), at 1.9 GHz under this load; the LDS pipe in 21 %, without a bank conflict.  A tile's results, which all CUs write
+// at about the same time, take a fifth of the time.  Small matrices are bound by the launches: 2 + 3 a step, 5.5 us each.
 // The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
 // multiplies.  Waves 4..7 ("late") run one phase behind waves 0..3: stage s is read in phases 2s and 2s + 1, its slot is
-// refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.
+// refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.  A phase
+// is short (32 products of 16 cycles), so what stands between two barriers beside them is kept small: 20 scalar
+// instructions in front of the products were 5 % of the whole.
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
     static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
     }
     // LATER: a slot is refilled a phase later than its last read (one phase less ahead), and no wait for that read stands in
     // front of the barrier: the products wait for their own operands as they come.  X' of pairs of ViT-L's matrices 1205 ->
-    // 1056 us, A 398 -> 385.  With two stages there is no phase to spare.
+    // 1056 us when it was built.  With two stages there is no phase to spare.
     constexpr bool LATER = S > 2;
     u32x4 fp[PP][MI], fq[QP][NI];
     int slot = 0;
@@ -706,8 +709,9 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
     }
     // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
     // the 256 CUs, a tile of 256 costing 256 a stage and one of 128, two of which share a CU and overlap their starts and
-    // ends, 83.  Measured, 256 against 128 (us, per launch): ViT-L's matrices (1440 / 5184 tiles) A 416 / 491, B 287 / 335,
-    // X' 650 / 889; ViT-S's (216 / 432) A 52 / 35, B 28 / 18, X' 36 / 35; 2048 x 2048 and the head's A 61 / 33, X' 57 / 46.
+    // ends, 83.  Measured, 256 against 128 (us, per launch): ViT-L's matrices A 371 / 391, B 219 / 231, X' 590 / 763, of pairs
+    // 1010 / 1300; ViT-S's A 46 / 31, B 22 / 15, X' 30 / 29, of pairs 51 / 49; the head MLP's A 52 / 24, X' 48 / 34, of pairs
+    // 83 / 42; one of 1024 x 588 and small ones A 30 / 13, X' 19 / 10.
     for (int kind = 0; kind < 2; ++kind) {
         double best = 0;
         for (int T = 256; T >= 128; T /= 2) {
