@@ -88,22 +88,38 @@ DEVI double block_sum_f64(double v, double* red) {
     return r;
 }
 
-// squares of rows [r0, r1): a wave a row; V elements a lane and load
+// squares of rows [r0, r1): V elements a thread and load, four loads in flight, rows one behind the other
 template <typename T, int V> DEVI double rows_sq(const T* p, int64_t ld, int cols, int r0, int r1) {
     typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T) * V)));
-    const int lane = threadIdx.x & 63;
+    const int g = (cols + V - 1) / V, dr = NTHR / g, dc = NTHR % g;         // vectors a row; a step of NTHR of them
+    int r = r0 + (int)threadIdx.x / g, c = (int)threadIdx.x % g;
     double s = 0;
-    for (int r = r0 + (threadIdx.x >> 6); r < r1; r += NTHR / 64) {
-        const T* x = p + r * ld;
-        for (int c = lane * V; c < cols; c += 64 * V) {
-            if (V == 1 || c + V <= cols) {
-                const vec v = *(const vec*)(x + c);
+    while (r < r1) {
+        float v[4][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) { const double d = (double)(float)v[i]; s = fma(d, d, s); }
-            } else {
-                for (int i = c; i < cols; ++i) { const double d = (double)(float)x[i]; s = fma(d, d, s); }
+        for (int u = 0; u < 4; ++u) {
+            const T* x = p + r * ld + c * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[u][i] = 0.f;
+            if (r < r1) {
+                if (V == 1 || c * V + V <= cols) {
+                    const vec w = *(const vec*)x;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[u][i] = (float)w[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (c * V + i < cols) v[u][i] = (float)x[i];
+                }
             }
+            r += dr;
+            c += dc;
+            if (c >= g) { c -= g; ++r; }
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < V; ++i) s = fma((double)v[u][i], (double)v[u][i], s);
     }
     return s;
 }
@@ -692,7 +708,10 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         q.mp = (int)up(q.m, 64);
         q.np = (int)up(q.n, 64);
         if ((int64_t)q.mp * q.np * 2 >= (1ll << 31)) return DINO_ERR_TOO_LARGE;
-        int64_t p = ((int64_t)q.m * q.n + 16383) / 16384;
+        // elements a workgroup of the norm: few where many would leave CUs idle (with 16384 throughout and one load in flight:
+        // one of 192 x 192 7 us, now 5; one of 1024 x 588 and small ones 12, now 5; the head MLP's 13, now 11)
+        const int64_t each = (int64_t)s.batch * q.m * q.n > (1 << 22) ? 16384 : 4096;
+        int64_t p = ((int64_t)q.m * q.n + each - 1) / each;
         if (p > 256) p = 256;
         q.parts = (int)(p > q.rows ? q.rows : p);
         const int64_t pt = (int64_t)((q.mp + 63) / 64) * ((q.np + 63) / 64);
