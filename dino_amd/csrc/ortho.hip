@@ -32,6 +32,7 @@ typedef __attribute__((address_space(3))) void* lptr_t;
 
 constexpr int BK = 32, NTHR = 256;
 constexpr int ITEMS = 16;                       // items described by one launch of the norm kernel
+constexpr int BLK = 6;                          // tiles' order: by blocks of 6 x 6
 constexpr float SX = 4096.f;                    // X is stored times this
 constexpr double SPLIT_ABOVE = 8.0;
 
@@ -151,15 +152,35 @@ __global__ __launch_bounds__(NTHR) void ortho_norm_kernel(const Setup su, const 
         const int u = sym ? t : t - q.batch * ns, mat = u / (sym ? ns : nr);
         int k = u - mat * (sym ? ns : nr);
         Tile d{q.xoff + (int64_t)mat * q.mp * q.np, q.aoff + (int64_t)mat * q.mp * q.mp, q.mp, q.np, 0, 0, id, mat, q.mat0 + mat, 0};
-        if (sym) {
-            int ti = 0;
-            while (k >= sm - ti) { k -= sm - ti; ++ti; }
-            d.m0 = ti * ws.tsym;
-            d.n0 = (ti + k) * ws.tsym;
+        // Tiles that follow each other, which the 32 CUs of one XCD take, share rows and columns in its L2 (the head MLP's 2048 x
+        // 2048: 455 us in all by whole rows, 446 by blocks; matrices of up to 6 tiles a side have the same order either way).
+        if (sym) {                           // BLK x BLK at a time
+            int r = 0, c = 0;
+            for (;;) {
+                const int h = min(BLK, sm - r), n = r == c ? h * (h + 1) / 2 : h * min(BLK, sm - c);
+                if (k < n) break;
+                k -= n;
+                c += BLK;
+                if (c >= sm) { r += BLK; c = r; }
+            }
+            if (r == c) {
+                const int h = min(BLK, sm - r);
+                int i = 0;
+                while (k >= h - i) { k -= h - i; ++i; }
+                r += i;
+                c += i + k;
+            } else {
+                const int w = min(BLK, sm - c);
+                r += k / w;
+                c += k % w;
+            }
+            d.m0 = r * ws.tsym;
+            d.n0 = c * ws.tsym;
             ws.sym[q.sym0 + u] = d;
-        } else {                             // one column panel after the other: it stays in L2
-            d.m0 = (k % rm) * ws.trect;
-            d.n0 = (k / rm) * ws.trect;
+        } else {                             // BLK rows of tiles at a time, column by column
+            const int rn = nr / rm, r = k / (BLK * rn) * BLK, h = min(BLK, rm - r), e = k - r * rn;
+            d.m0 = (r + e % h) * ws.trect;
+            d.n0 = (e / h) * ws.trect;
             ws.rect[q.rect0 + u] = d;
         }
     }
