@@ -281,7 +281,7 @@ struct GemmArgs {
 DEVI int fsw(int x) { return (4 - (x & 3)) & 3; }
 template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// T x T tiles of a product, a workgroup of eight waves (2 x 4, each T/2 x T/4) walking its share of them.
+// T x T tiles of a product, a workgroup of eight waves (2 x 4, each T/2 x T/4; T = 64: 4 x 2) walking its share of them.
 //   GRAM    A = X X^T               rows of X against rows of X; tiles on and above the diagonal, written twice
 //   POLY    B = a I + b A + c A A   A symmetric: rows against rows again
 //   UPDATE  X' = B X                rows of B against COLUMNS of X (transposing LDS reads)
@@ -301,17 +301,19 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 // instructions in front of the products were 5 % of the whole.
 enum { GRAM, POLY, UPDATE, FINAL };
 template <int T, bool SPLIT> struct Cfg {
-    static constexpr int MI = T / 32, NI = T / 64;                  // fragments of 16 x 16 a wave
-    // parts of a stage: KB panels of P and of Q (SPLIT: Q's hi, then its lo).  Two panels for T = 128: half the phases,
-    // whose fixed part (barrier, LDS latency: about 0.35 us) is otherwise longer than their products
-    static constexpr int KB = T == 128 ? 2 : 1, PP = KB, QP = SPLIT ? 2 * KB : KB;
+    static constexpr int WM = T == 64 ? 4 : 2, WN = 8 / WM;         // waves along rows and columns
+    static constexpr int MI = T / 16 / WM, NI = T / 16 / WN;        // fragments of 16 x 16 a wave
+    // parts of a stage: KB panels of P and of Q (SPLIT: Q's hi, then its lo).  Two panels for T <= 128: half the phases,
+    // whose fixed part (barrier, LDS latency: about 0.25 us) is otherwise longer than their products
+    static constexpr int KB = T <= 128 ? 2 : 1, PP = KB, QP = SPLIT ? 2 * KB : KB;
     static constexpr int OPB = T * BK * 2, STAGE = (PP + QP) * OPB;
-    static constexpr int S = SPLIT ? 3 : T == 256 ? 4 : 2;
-    static constexpr int ND = T / 128;                              // DMAs a wave and part
+    static constexpr int S = T == 128 ? (SPLIT ? 3 : 2) : SPLIT && T == 256 ? 3 : 4;
+    static constexpr int PIECES = T / 16;                           // DMAs a part, of 16 rows of P each
+    static constexpr int NP = PP * PIECES / 8, NQ = QP * PIECES / 8;    // ... a wave and stage
     static constexpr int SUBM = 16 * MI, SUBN = 16 * NI;            // a wave's part of the tile
     static constexpr int IMG = SPLIT ? 0 : 16 * SUBM * 2;           // image of 16 columns of it (UPDATE has none)
-    static constexpr int SMEM = S * STAGE + 8 * IMG;                // 160 KB (SPLIT: 144), T = 128 without SPLIT 80 KB
-    static constexpr int PER_CU = T == 128 && !SPLIT ? 2 : 1;       // workgroups a CU: LDS and registers allow so many
+    static constexpr int SMEM = S * STAGE + 8 * IMG;                // T = 256: 160 KB (SPLIT: 144), 128: 80 (144), 64: 68 (96)
+    static constexpr int PER_CU = T <= 128 && !SPLIT ? 2 : 1;       // workgroups a CU: LDS and registers allow so many
 };
 // The DMA is written in assembly: behind the builtin the compiler waits for ALL requests before every transposing LDS
 // read, which may alias what is being filled for all it knows.  It has no register result; the waits are landed()'s.
@@ -366,11 +368,11 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Cfg<T, SPLIT> C;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
-    constexpr int S = C::S, MI = C::MI, NI = C::NI, ND = C::ND, KB = C::KB, PP = C::PP, QP = C::QP;
+    constexpr int S = C::S, MI = C::MI, NI = C::NI, KB = C::KB, PP = C::PP, QP = C::QP, NP = C::NP, NQ = C::NQ;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 2, wn = wave & 3, i = lane & 15, g = lane >> 4;
+    const int wm = wave / C::WN, wn = wave % C::WN, i = lane & 15, g = lane >> 4;
     int late = wave >> 2;
     asm volatile("" : "+s"(late));             // (an integer to the compiler, compared by scalar instructions)
     const Ws& ws = ga.ws;
@@ -385,10 +387,12 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
     // in a bank.  Rows behind the matrix read zeros or the next panel, panels behind it the last one: only their own
     // results, which are not stored, see them.  (A request never starts behind its buffer: the range check subtracts the
     // uniform part of the offset from the size.)  A wave moves pieces wave, wave + 8, ...: first P's, then Q's.
+    // Piece e = wave + 8 n of an operand is piece e % PIECES of its part e / PIECES.
+    constexpr int ND = C::PIECES >= 8 ? C::PIECES / 8 : 1;   // different pieces of a part that a wave takes
     int voP[ND], voQ[ND];
 #pragma unroll
     for (int u = 0; u < ND; ++u) {
-        const int e = wave + 8 * u, r = e * 16 + (lane >> 2), t = (e & 1) * 16 + (lane >> 2);
+        const int e = (wave + 8 * u) % C::PIECES, r = e * 16 + (lane >> 2), t = (e & 1) * 16 + (lane >> 2);
         voP[u] = r * 64 + (((lane & 3) ^ fsw(r >> 2)) << 4);
         voQ[u] = SYM ? voP[u] : t * 64 + (((lane & 3) ^ tkey(t)) << 4);
     }
@@ -404,7 +408,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         soP = tn.m0 * 64;
 #pragma unroll
         for (int u = 0; u < ND; ++u)
-            soQ[u] = SYM ? tn.n0 * 64 : min((tn.n0 >> 5) + ((wave + 8 * u) >> 1), (tn.np >> 5) - 1) * panel;
+            soQ[u] = SYM ? tn.n0 * 64 : min((tn.n0 >> 5) + (((wave + 8 * u) % C::PIECES) >> 1), (tn.np >> 5) - 1) * panel;
         left = (MODE == GRAM ? tn.np : tn.mp) / (BK * KB);
         rsP = rsrc(MODE == GRAM ? ws.x[ga.src][0] + tn.xo : MODE == POLY ? ws.a + tn.ao : ws.b + tn.ao,
                    tn.mp * (MODE == GRAM ? tn.np : tn.mp) * 2);
@@ -414,15 +418,18 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
         if (ji + 1 < nmine) tn = load_tile(tiles + b0 + (ji + 1) * G);
     };
     open();
-    constexpr int NREQ = (PP + QP) * ND;                   // requests of a wave and stage
+    constexpr int NREQ = NP + NQ;                          // requests of a wave and stage
+    static_assert(QP * MI >= NREQ, "multiply() takes one request a row");
+    auto part_of = [&](int n) { return C::PIECES >= 8 ? 8 * n / C::PIECES : (wave + 8 * n) / C::PIECES; };
     auto request = [&](int n) {
-        const int u = n % ND;
-        if (n < PP * ND) {
-            const int h = n / ND;
-            dma16(iat + h * C::OPB + u * 8192, voP[u], rsP, soP + h * panel);
+        if (n < NP) {
+            const int h = part_of(n);
+            dma16(iat + n * 8192, voP[n % ND], rsP, soP + h * panel);
         } else {
-            const int h = n / ND - PP;                     // (h % KB: panel along the contraction)
-            dma16(iat + (PP + h) * C::OPB + u * 8192, voQ[u], rsQ[SPLIT ? h / KB : 0], soQ[u] + (h % KB) * (SYM ? panel : 2048));
+            n -= NP;
+            const int h = part_of(n);                      // (h % KB: panel along the contraction)
+            dma16(iat + PP * C::OPB + n * 8192, voQ[n % ND], rsQ[SPLIT ? 8 * n / (C::PIECES * KB) : 0],
+                  soQ[n % ND] + (h % KB) * (SYM ? panel : 2048));
         }
     };
     // (Behind the last tile the requests go on, to the last matrix's first rows: a stage is always NREQ of them.)
@@ -506,6 +513,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
                 if (n < NREQ && req) request(n);
                 if (n == NREQ && req) requested();
             }
+        if (QP * MI == NREQ && req) requested();
     };
     auto phase = [&]() {
         asm volatile("" ::: "memory");
@@ -536,7 +544,7 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
             // (loads without a branch, so that they are in flight together: a fragment behind the matrix reads another one or
             // zero and is not stored)
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(ws.a + d.ao), 0, mp * mp * 2, 0x00020000);
-            constexpr int PART = MI / 2;
+            constexpr int PART = (MI + 1) / 2;
 #pragma unroll
             for (int q = 0; q < MI; q += PART) {
                 u32x4 el[PART][NI / 2];
@@ -613,9 +621,10 @@ __global__ __launch_bounds__(512, (2 * Cfg<T, SPLIT>::PER_CU)) void ortho_gemm_k
                     *(unsigned*)(img + at(c + 1, m)) = odd ? pack2<TOBF>(x1, v[3]) : pack2<TOBF>(v[1], x1);
                 }
                 for (int e = lane; e < 2 * C::SUBM; e += 64) {
-                    // panels: 64 bytes of each of the 16 columns; else whole columns
-                    const int c = TOBF ? e / (C::SUBM / 8) : (e >> 2) & 15;
-                    const int m = TOBF ? (e - c * (C::SUBM / 8)) * 8 : (e >> 6) * 32 + (e & 3) * 8;
+                    // panels: up to 64 bytes of each of the 16 columns; else whole columns
+                    constexpr int CH = C::SUBM < 32 ? C::SUBM / 8 : 4;
+                    const int c = TOBF ? e / (C::SUBM / 8) : (e / CH) & 15;
+                    const int m = TOBF ? (e - c * (C::SUBM / 8)) * 8 : e / (16 * CH) * 32 + e % CH * 8;
                     const u32x4 w = *(const u32x4*)(img + at(c, m));
                     const int dr = wn0 + ni * 16 + c, dc = wm0 + m;
                     if (dr >= rows || dc >= cols) continue;
@@ -748,13 +757,15 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         if (out) out[i] = q;
     }
     // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
-    // the 256 CUs, a tile of 256 costing 256 a stage and one of 128, two of which share a CU and overlap their starts and
-    // ends, 83.  Measured, 256 against 128 (us, per launch): ViT-L's matrices A 371 / 391, B 219 / 231, X' 590 / 763, of pairs
-    // 1010 / 1300; ViT-S's A 46 / 31, B 22 / 15, X' 30 / 29, of pairs 51 / 49; the head MLP's A 52 / 24, X' 48 / 34, of pairs
-    // 83 / 42; one of 1024 x 588 and small ones A 30 / 13, X' 19 / 10.
+    // the 256 CUs, a tile of 256 costing 256 a stage, one of 128 (two share a CU and overlap their starts and ends) 83, one of
+    // 64 45: it has the shorter phases, but reads twice as much for a product as one of 128.  So 64 is taken where all of
+    // them run at once.  Measured (us): a launch with 256 / 128: ViT-L's matrices A 371 / 391, B 219 / 231, X' 590 / 763,
+    // of pairs 1010 / 1300; ViT-S's A 46 / 31, B 22 / 15, X' 30 / 29, of pairs 51 / 49; the head MLP's A 52 / 24, X' 48 / 34, of
+    // pairs 83 / 42.  A launch with 128 / 64: one of 192 x 192 5.5 / 4.4; one of 1024 x 588 and small ones A 13 / 8, B 11 / 6;
+    // the head's A 24 / 33; ViT-S's X' 31 / 45.  A whole call: one of 1024 x 1024 225 / 145, of 512 x 512 147 / 100.
     for (int kind = 0; kind < 2; ++kind) {
         double best = 0;
-        for (int T = 256; T >= 128; T /= 2) {
+        for (int T = 256; T >= 64; T /= 2) {
             double work = 0, tiles = 0;
             for (int i = 0; i < count; ++i) {
                 const int64_t m = up(items[i].rows < items[i].cols ? items[i].rows : items[i].cols, 64);
@@ -765,7 +776,7 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
                 work += k * (double)(kind ? m : n + m);
             }
             if (tiles == 0) tiles = 1;
-            const double cost = work / tiles * ceil(tiles / 256) * (T == 256 ? 256 : 83);
+            const double cost = work / tiles * ceil(tiles / 256) * (T == 256 ? 256 : T == 128 ? 83 : 45);
             if (T == 256 || cost < best) { best = cost; L.tile[kind] = T; }
         }
     }
@@ -830,8 +841,9 @@ template <int MODE, int T, bool SPLIT> int launch_as(const GemmArgs& ga, hipStre
 }
 template <int MODE> int launch_gemm(GemmArgs& ga, int T, bool split, int64_t tiles, hipStream_t st) {
     ga.ntiles = (int)tiles;
-    if (MODE == UPDATE && split) return T == 256 ? launch_as<UPDATE, 256, true>(ga, st) : launch_as<UPDATE, 128, true>(ga, st);
-    return T == 256 ? launch_as<MODE, 256, false>(ga, st) : launch_as<MODE, 128, false>(ga, st);
+    if (MODE == UPDATE && split)
+        return T == 256 ? launch_as<UPDATE, 256, true>(ga, st) : T == 128 ? launch_as<UPDATE, 128, true>(ga, st) : launch_as<UPDATE, 64, true>(ga, st);
+    return T == 256 ? launch_as<MODE, 256, false>(ga, st) : T == 128 ? launch_as<MODE, 128, false>(ga, st) : launch_as<MODE, 64, false>(ga, st);
 }
 
 }  // namespace

@@ -128,6 +128,21 @@ def test_scale_of_the_update(scale):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(2, 1000, 1030), (2, 1030, 1000), (10, 450, 1500)])
+def test_middle_tiles_with_tiny_matrices_beside_them(shape):
+    """Enough work for the 128 x 128 tiles (and, for the last, 64 x 64 ones beside them)."""
+    big = momentum(shape, 12)
+    small = [momentum((3, 5, 7), 1), momentum((65, 129), 3)]
+    got = ops.orthogonalize([big.cuda()] + [u.cuda() for u in small])
+    for i in (0, shape[0] - 1):
+        off(got[0][i], big[i])
+    for u, o in zip(small, got[1:]):
+        for a, b in zip(u.reshape(-1, *u.shape[-2:]), o.reshape(-1, *o.shape[-2:])):
+            off(b, a)
+    assert torch.equal(ops.orthogonalize(big.cuda()), got[0])
+
+
+@gpu
 @pytest.mark.parametrize("shape", [(32704, 32768), (32768, 16400)])
 def test_largest_matrices(shape):
     """Offsets up to the last byte that a matrix may have (2^31).  Zeros but for blocks in the corners and between: rows and
