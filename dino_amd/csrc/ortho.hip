@@ -814,13 +814,24 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
     return DINO_OK;
 }
 
-// largest |p(x)| and |a + b x^2 + c x^4| over singular values up to `top`
-void poly_bounds(const float* c, double top, double& px, double& qx) {
+// largest |p(x)| and |q| over singular values x up to `top`,  p = x q,  q = a + b x^2 + c x^4: at the ends or where a
+// derivative is 0  (q' = 2 x (b + 2 c y),  p' = a + 3 b y + 5 c y^2,  y = x^2)
+void poly_bounds(const float* co, double top, double& px, double& qx) {
+    const double a = co[0], b = co[1], c = co[2], end = top * top, disc = 9 * b * b - 20 * a * c;
+    double y[5] = {0, end, -1, -1, -1};
+    if (c != 0) {
+        y[2] = -b / (2 * c);
+        if (disc >= 0) {
+            y[3] = (-3 * b + sqrt(disc)) / (10 * c);
+            y[4] = (-3 * b - sqrt(disc)) / (10 * c);
+        }
+    } else if (b != 0) y[3] = -a / (3 * b);
     px = qx = 0;
-    for (int k = 0; k <= 512; ++k) {
-        const double x = top * k / 512, x2 = x * x, q = c[0] + c[1] * x2 + c[2] * x2 * x2;
-        px = fmax(px, fabs(q * x));
-        qx = fmax(qx, fabs(q));
+    for (double v : y) {
+        if (!(v >= 0 && v <= end)) continue;
+        const double q = fabs(a + b * v + c * v * v);
+        px = fmax(px, q * sqrt(v));
+        qx = fmax(qx, q);
     }
 }
 

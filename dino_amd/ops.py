@@ -613,9 +613,8 @@ class OrthoPlan:
         _req(len(set(given)) == len(given), "out: one tensor twice")
         self.out, self._updates, self._steps, self._eps = [], ups, steps, float(eps)
         self._coeffs = (ctypes.c_float * (3 * steps))(*[float(v) for c in rows for v in c])
-        # (no items: the checks of steps and coefficients only)
-        check(_lib.load().dino_ortho(None, 0, steps, self._coeffs, self._eps, None, 0, None), "dino_ortho")
-        if not ups:
+        if not ups:                        # (the checks of steps and coefficients, which run() has for others)
+            check(_lib.load().dino_ortho(None, 0, steps, self._coeffs, self._eps, None, 0, None), "dino_ortho")
             return
         _dev(*ups, *outs)
         self._dev = dev = ups[0].device
