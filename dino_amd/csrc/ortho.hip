@@ -293,7 +293,8 @@ template <int N> DEVI void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"
 // What bounds it, for X' of ViT-L's 144 matrices (0.62 TFLOP; 0.9 GB to read, 0.6 GB to write): 590 us = 1050 TFLOP/s (a large
 // library product reaches 1306 here); of pairs (1.24 TFLOP) 1030 us = 1200.  The matrix pipes are busy in 57 % of the cycles (pairs:
 // 66 %), at 1.9 GHz under this load; a stage's fragments and DMAs are 128 KB of LDS, without a bank conflict, as long at 128
-// bytes a cycle as its products.  A tile's results, which all CUs write at about the same time, take a fifth of the time.  Small matrices are bound by the launches: 2 + 3 a step, 4.2 us each.
+// bytes a cycle as its products.  A tile's results, which all CUs write at about the same time, take a fifth of the time.
+// Small matrices are bound by the launches: 2 + 3 a step, 4.2 us each.
 // The two waves of a SIMD work in opposite phases, a barrier apart: one reads its fragments from LDS while the other
 // multiplies.  Waves 4..7 ("late") run one phase behind waves 0..3: stage s is read in phases 2s and 2s + 1, its slot is
 // refilled from phase 2s + 2 on, and both groups write a finished tile's results in the phase after its last read.  A phase
