@@ -758,12 +758,13 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
         if (out) out[i] = q;
     }
     // Tile size of the symmetric products and of the update, each the one of least estimated time: rounds of tiles over
-    // the 256 CUs, a tile of 256 costing 256 a stage, one of 128 (two share a CU and overlap their starts and ends) 83, one of
-    // 64 45: it has the shorter phases, but reads twice as much for a product as one of 128.  So 64 is taken where all of
-    // them run at once.  Measured (us): a launch with 256 / 128: ViT-L's matrices A 371 / 391, B 219 / 231, X' 590 / 763,
+    // the 256 CUs, a tile of 256 costing 256 a stage, one of 128 (two share a CU and overlap their starts and ends) 83.  Tiles of
+    // 64 have the shorter phases, but read twice as much for a product; two of them on a CU cost 53 (symmetric: less of the
+    // matrix twice) or 78.  So 64 is taken where all of them run at once.  Measured (us): a launch with 256 / 128: ViT-L's matrices A 371 / 391, B 219 / 231, X' 590 / 763,
     // of pairs 1010 / 1300; ViT-S's A 46 / 31, B 22 / 15, X' 30 / 29, of pairs 51 / 49; the head MLP's A 52 / 24, X' 48 / 34, of
     // pairs 83 / 42.  A launch with 128 / 64: one of 192 x 192 5.5 / 4.4; one of 1024 x 588 and small ones A 13 / 8, B 11 / 6;
-    // the head's A 24 / 33; ViT-S's X' 31 / 45.  A whole call: one of 1024 x 1024 225 / 145, of 512 x 512 147 / 100.
+    // the head's A 24 / 33; ViT-S's X' 31 / 45.  A whole call: one of 1024 x 1024 225 / 145, of 512 x 512 147 / 100,
+    // 48 of 192 x 192 and 24 of 768 x 192 172 / 154 (64 for A and B only), 24 and 12 of 384 292 / 324.
     for (int kind = 0; kind < 2; ++kind) {
         double best = 0;
         for (int T = 256; T >= 64; T /= 2) {
@@ -777,7 +778,7 @@ int describe(const dino_ortho_item* items, int count, Mat* out, Layout& L) {
                 work += k * (double)(kind ? m : n + m);
             }
             if (tiles == 0) tiles = 1;
-            const double cost = work / tiles * ceil(tiles / 256) * (T == 256 ? 256 : T == 128 ? 83 : 45);
+            const double cost = work / tiles * (T == 64 ? ceil(tiles / 512) * (kind ? 78 : 53) : ceil(tiles / 256) * (T == 256 ? 256 : 83));
             if (T == 256 || cost < best) { best = cost; L.tile[kind] = T; }
         }
     }

@@ -68,7 +68,7 @@ def train_one_epoch(student, teacher, teacher_without_ddp, dino_loss, data_loade
     """Reference signature (train_utils.py:14-36).  fp16_scaler is accepted and ignored: the
     bf16 path needs no loss scaling.  The adversarial branch is out of scope.
     watch_every > 0: every so many steps DINOLoss.watch is taken too, and its averages over them join the returned
-    stats."""
+    stats (it needs the student's logits: not together with fused_head_loss)."""
     if domain_classifier is not None:
         raise NotImplementedError("domain-adversarial branch (adversarial.enable) is out of scope")
     if distributed.is_enabled() and hasattr(data_loader, "sampler") and hasattr(data_loader.sampler, "set_epoch"):

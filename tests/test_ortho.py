@@ -128,7 +128,7 @@ def test_scale_of_the_update(scale):
 
 
 @gpu
-@pytest.mark.parametrize("shape", [(2, 1000, 1030), (2, 1030, 1000), (10, 450, 1500)])
+@pytest.mark.parametrize("shape", [(4, 1000, 1030), (4, 1030, 1000), (2, 1000, 1030), (10, 450, 1500)])
 def test_middle_tiles_with_tiny_matrices_beside_them(shape):
     """Enough work for the 128 x 128 tiles (and, for the last, 64 x 64 ones beside them)."""
     big = momentum(shape, 12)
