@@ -136,8 +136,10 @@ DEVI void put_top(const FwdArgs& a, int64_t row, int j, u64 key, float md, float
 // One workgroup of NT threads takes one chunk (at most NT * 8 * NV columns) of one row, held in registers: read
 // once, then the maximum, the sums and the best k come from registers.
 // Bound: memory, with about 12 vector instructions and an exp2 an element close behind (50 us of the 85 below).  MI355X:
-// 2560 rows of 65536 bf16 (336 MB) 80 .. 86 us = 4.0 TB/s; 512 of them with a centre (it stays in L2) and 8 best (67 MB)
-// 24 us = 2.8 TB/s; 12608 of 4096 with 2 best (103 MB) 25 us = 4.1 TB/s; 333 fp32 rows of 8191, a third of them -inf, 9.7 us.
+// 2560 rows of 65536 bf16 (336 MB) 59 us one call after another = 5.7 TB/s, 80 .. 86 beside the gradient's writes; with a centre,
+// read from L2 by every workgroup, 91.  Best prototypes: one 3 us more, eight 24 (their lower bound and the list of candidates are
+// 200 instructions a wave).  512 rows with a centre and 8 best 22 us + the join; 12608 of 4096 with 2 best (103 MB) 25 us =
+// 4.1 TB/s; 333 fp32 rows of 8191, a third of them -inf, 9.7 us.
 // Splitting a row over workgroups of 256 threads leaves 32 values a thread in registers, five waves a SIMD or more.
 template <typename T, int NT, int NV, bool CEN>
 __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
@@ -250,23 +252,26 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
 
     if (a.topk > 0) {
         const int k = a.topk;
-        // lower bound of the k-th best: the k-th best of a wave's 64 thread maxima (16 leading bits of the order,
-        // by bisection over ballots), the larger of the waves'
-        const unsigned key16 = ord_bits(tm) >> 16;
-        unsigned th = 0;
-#pragma unroll
-        for (int b = 15; b >= 0; --b) {
-            const unsigned c = th | (1u << b);
-            if (__popcll(__ballot(key16 >= c)) >= k) th = c;
-        }
+        // lower bound of the k-th best: the maximum itself for one; else the k-th best of a wave's 64 thread maxima (16 leading
+        // bits of the order, by bisection over ballots), the larger of the waves'
+        float T_ = md;
         __syncthreads();
-        if (NW > 1) {
-            if (lane == 0) red[wave] = __builtin_bit_cast(float, th);
-            __syncthreads();
+        if (k > 1) {
+            const unsigned key16 = ord_bits(tm) >> 16;
+            unsigned th = 0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) th = max(th, __builtin_bit_cast(unsigned, red[w]));
+            for (int b = 15; b >= 0; --b) {
+                const unsigned c = th | (1u << b);
+                if (__popcll(__ballot(key16 >= c)) >= k) th = c;
+            }
+            if (NW > 1) {
+                if (lane == 0) red[wave] = __builtin_bit_cast(float, th);
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < NW; ++w) th = max(th, __builtin_bit_cast(unsigned, red[w]));
+            }
+            T_ = th <= 0x007Fu ? NEG_INF : ord_float(th << 16);
         }
-        const float T_ = th <= 0x007Fu ? NEG_INF : ord_float(th << 16);
         const bool nan = s != s;             // a NaN is no maximum of its vector: such a chunk takes the rounds below
         // (columns behind the chunk's end hold -inf and are told by their index)
 #pragma unroll
@@ -339,13 +344,22 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const FwdArgs a) {
     }
 }
 
-// joins the chunks of a row: one wave per row, lane = chunk (at most 64).  4 .. 6 us: latency of the launch and of topk
-// rounds over the chunks' sorted keys.
+// Joins the chunks of a row: one wave per row, lane = chunk (at most 64).  Up to 64 keys are ranked against each other, a key a
+// lane; more are merged, a round a result (ranked too, 160 took 6.6 us instead of 4).  4 .. 5 us, a launch's latency (512 rows of
+// 8 chunks with 8 best each: 6 by rounds).
 template <typename T> __global__ __launch_bounds__(64) void logprob_join_kernel(const FwdArgs a) {
+    __shared__ u64 all[64];
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
+    const int n = a.S * a.topk;
+    const u64* keys = a.keys + row * n;
     Part q{NEG_INF, 0.f, 0.f, 0.f};
     if (lane < a.S) q = a.parts[row * a.S + lane];
+    u64 cur = 0;
+    if (n <= 64) {
+        if (lane < n) cur = keys[lane];
+        all[lane] = cur;
+    }
     const float md = wave_max(q.m);
     const float sc = a.inv_temp * LOG2E;
     const float dl = q.m == NEG_INF ? 0.f : (q.m - md) * sc;       // an empty chunk has s = t = 0 (or NaN)
@@ -353,9 +367,17 @@ template <typename T> __global__ __launch_bounds__(64) void logprob_join_kernel(
     const float s = wave_sum(q.s * f);
     const float t2 = wave_sum(f * fmaf(q.s, fmaxf(dl, Z_MIN), q.t));
     finish_row<T>(a, row, md, s, t2, lane);
+    if (n <= 64) {
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 8
+        for (int r = 0; r < n; ++r) rank += all[r] > cur;
+        if (cur && rank < a.topk) put_top(a, row, rank, cur, md, s);       // (0: no key, a chunk of fewer columns)
+        return;
+    }
     int head = 0;
-    const u64* keys = a.keys + (row * a.S + lane) * a.topk;
-    u64 cur = lane < a.S && a.topk > 0 ? keys[0] : 0;
+    keys += lane * a.topk;
+    if (lane < a.S) cur = keys[0];
     for (int j = 0; j < a.topk; ++j) {
         const u64 b = wave_max_u64(cur);
         if (cur == b && b != 0) {
